@@ -252,6 +252,27 @@ int mk_gemm(int in_type, int epi, const void* A, int lda, const void* B, int ldb
 /* Last-token LM head: logits (B, V) f32 = hidden (B, H) bf16 @ lm_head (V, H)^T, any B. */
 int mk_lm_head(const void* hidden, const void* lm_head, int B, int H, int V, float* logits, void* stream);
 
+/* Log probabilities of rows of logits (T, V), row stride ld elements, MK_LOGITS_* type; no counterpart in the
+ * reference, whose answers vLLM's sampler turns into log probabilities.  With x a row in f32, m = max x and
+ * S = sum exp(x - m):
+ *   lse = m + ln S;  entropy = ln S - sum exp(x - m) (x - m) / S  (nats; both (T))
+ *   token_lp (T, n_ids) = (x[id] - m) - ln S of the given tokens ids (T, n_ids), int32 or int64 (ids64 != 0)
+ *   ranks (T, n_ids) = 1 + the number of tokens before id in the order (logit descending, index ascending)
+ *   top_lp, top_ids (T, top): the first `top` tokens of that order
+ * An id outside [0, V) has log probability -inf and rank -1.  A row of nothing but -inf has lse and log
+ * probabilities -inf and entropy 0.  A row with a NaN or +inf has no distribution: its numbers are NaN, its ranks
+ * and top_ids -1.  n_ids and top may be 0 (at most MK_LOGPROBS_MAX each, top <= V), their pointers are then unused.
+ * Any alignment and stride of whole elements.  scratch: mk_logprobs_scratch_bytes bytes, 16-byte aligned (may be
+ * 0 bytes); calls that share one scratch buffer must not overlap.  Results do not depend on timing. */
+#define MK_LOGITS_F32 0
+#define MK_LOGITS_BF16 1
+#define MK_LOGITS_F16 2
+#define MK_LOGPROBS_MAX 64
+size_t mk_logprobs_scratch_bytes(int T, int V, int n_ids, int top);
+int mk_logprobs(const void* logits, int type, size_t ld, int T, int V, const void* ids, int ids64, int n_ids, int top,
+                float* token_lp, int32_t* ranks, float* top_lp, int32_t* top_ids, float* entropy, float* lse,
+                void* scratch, size_t scratch_bytes, void* stream);
+
 /* Weight preparation on the GPU: the per-parameter work of prepare_mk_weights (mk_weights.py:113-123,
  * :229-252), bit-identical to the CPU restatement; the small FP32 calibration forward stays on the host.
  * w is an HF linear weight (n_out, n_in) bf16 and W = w^T * fold its (in, out) f32 view (fold = 1/sqrt(hd)

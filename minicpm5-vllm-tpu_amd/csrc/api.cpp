@@ -332,6 +332,35 @@ int mk_lm_head(const void* hidden, const void* lm_head, int B, int H, int V, flo
   MK_TRY(mk::launch_lm_head(g, static_cast<hipStream_t>(stream)));
 }
 
+size_t mk_logprobs_scratch_bytes(int T, int V, int n_ids, int top) {
+  if (T < 1 || V < 1 || n_ids < 0 || top < 0) return 0;
+  return mk::logprob_scratch_bytes(T, V, n_ids, top);
+}
+
+int mk_logprobs(const void* logits, int type, size_t ld, int T, int V, const void* ids, int ids64, int n_ids, int top,
+                float* token_lp, int32_t* ranks, float* top_lp, int32_t* top_ids, float* entropy, float* lse,
+                void* scratch, size_t scratch_bytes, void* stream) {
+  MK_REQUIRE(type >= MK_LOGITS_F32 && type <= MK_LOGITS_F16, "logprobs: unknown logits type");
+  MK_REQUIRE(T >= 0 && V >= 1 && V <= (1 << 30), "logprobs: T must be >= 0 and V in 1 .. 2^30");
+  MK_REQUIRE(n_ids >= 0 && n_ids <= mk::LP_MAX_IDS, "logprobs: at most 64 given tokens a row");
+  MK_REQUIRE(top >= 0 && top <= mk::LP_MAX_TOP && top <= V, "logprobs: top must be in 0 .. min(64, V)");
+  MK_REQUIRE(ld >= (size_t)V || T <= 1, "logprobs: row stride below V");
+  if (T == 0) return MK_OK;
+  MK_REQUIRE(logits && entropy && lse, "logprobs: null pointer");
+  MK_REQUIRE(n_ids == 0 || (ids && token_lp && ranks), "logprobs: null pointer of the given tokens");
+  MK_REQUIRE(top == 0 || (top_lp && top_ids), "logprobs: null pointer of the alternatives");
+  MK_REQUIRE((uintptr_t)logits % (type == MK_LOGITS_F32 ? 4 : 2) == 0, "logprobs: logits not aligned to an element");
+  const size_t need = mk::logprob_scratch_bytes(T, V, n_ids, top);
+  if (scratch_bytes < need || (need && !scratch)) {
+    mk::set_error("logprobs: scratch too small");
+    return MK_ENOMEM;
+  }
+  MK_REQUIRE(!need || aligned16(scratch), "logprobs: scratch must be 16-byte aligned");
+  const mk::LogprobArgs a{logits,   ld,    type,   ids,     ids64 != 0, n_ids, T, V, top,
+                          token_lp, ranks, top_lp, top_ids, entropy,    lse};
+  MK_TRY(mk::launch_logprobs(a, scratch, static_cast<hipStream_t>(stream)));
+}
+
 int mk_pack_weight(const void* in, int ld_in, void* out, int K, int N, int elem_bytes, int map, int ic, int inter,
                    void* stream) {
   mk::PackArgs p{};

@@ -104,6 +104,27 @@ int launch_gemm_skinny(const GemmArgs& g, hipStream_t st);
 // Logits (F32 epilogue, bf16 operands) of any number of rows, the weights read once per 64 of them.
 int launch_lm_head(const GemmArgs& g, hipStream_t st);
 
+// ------------------------------------------------------------------------------ log probabilities
+// Rows x (T, V) at row stride ldx (elements): log p of n_ids given tokens a row with their ranks, entropy, log of the
+// sum of exponentials, and the `top` best alternatives (logprobs.hip).
+constexpr int LP_MAX_IDS = 64, LP_MAX_TOP = 64;
+struct LogprobArgs {
+  const void* x;
+  size_t ldx;
+  int dtype;             // of x: 0 f32, 1 bf16, 2 f16
+  const void* ids;       // (T, n_ids) int32, or int64 with ids64
+  int ids64, n_ids;
+  int T, V, top;
+  float* token_lp;       // (T, n_ids)
+  int* ranks;            // (T, n_ids)
+  float* top_lp;         // (T, top)
+  int* top_ids;          // (T, top)
+  float* entropy;        // (T)
+  float* lse;            // (T)
+};
+size_t logprob_scratch_bytes(int T, int V, int n_ids, int top);
+int launch_logprobs(const LogprobArgs& a, void* ws, hipStream_t st);
+
 // ------------------------------------------------------------------------------ norm / quant
 // Activation quantisation of rows x (T, H), one kernel for the reference's four activation modes
 // (qmax = 127 for int8, 448 for fp8 e4m3; rstd = rsqrt(mean(x^2) + eps) with norm, else 1):

@@ -138,4 +138,12 @@ inline bool lm_head_skinny(int rows, int V, int K) {
   return K > 1536 && (rows == 1 || (rows == 2 && V >= 3 * 128 * 256));
 }
 
+// Workgroups that share a row of the log-probability pass: one per row once the rows fill the 256 CUs, else enough for
+// four a CU, each with a whole 1024-value tile for each of its 4 waves.
+inline int logprob_splits(int T, int V) {
+  const int most = (V + 4095) / 4096, want = (1024 + T - 1) / T;
+  if (T >= 256 || most <= 1) return 1;
+  return want < most ? want : most;
+}
+
 }  // namespace mk

@@ -6,7 +6,9 @@ kernels.  Each wrapper checks dtypes, devices, contiguity and shapes on the host
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -37,6 +39,31 @@ def _need(t: torch.Tensor, name: str, dtype=None, shape=None):
         raise MkError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.data_ptr() % 16:
         raise MkError(f"{name}: must be 16-byte aligned")
+
+
+def _need_rows(t: torch.Tensor, name: str, dtypes, cols: int | None = None):
+    """A (rows, cols) GPU tensor of one of `dtypes` whose rows are contiguous, at any row stride and alignment."""
+    if not isinstance(t, torch.Tensor):
+        raise MkError(f"{name}: expected a torch.Tensor")
+    if not t.is_cuda:
+        raise MkError(f"{name}: must be a GPU tensor (libmk has no CPU path)")
+    if t.dim() != 2 or t.dtype not in dtypes:
+        raise MkError(f"{name}: {tuple(t.shape)} {t.dtype}, expected 2 dimensions of {' / '.join(str(d) for d in dtypes)}")
+    if cols is not None and t.shape[1] != cols:
+        raise MkError(f"{name}: {t.shape[1]} columns, expected {cols}")
+    if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+        raise MkError(f"{name}: rows must be contiguous and must not overlap")
+
+
+def _same_device(t: torch.Tensor, **others):
+    for name, o in others.items():
+        if o is not None and o.device != t.device:
+            raise MkError(f"{name}: on {o.device}, expected {t.device}")
+
+
+def _on(t: torch.Tensor):
+    """Makes t's device the current one, so that its stream, allocations and launches are that device's."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def attn_scratch_bytes(B: int, S: int, n_kv: int, head_dim: int) -> int:
@@ -159,6 +186,69 @@ def lm_head(hidden: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     return out
 
 
+class LogProbs(NamedTuple):
+    """Log probabilities of T rows (nats, f32).  ids None: no token_logprobs / ranks; top 0: no top_*."""
+    token_logprobs: torch.Tensor | None   # of ids' shape
+    ranks: torch.Tensor | None            # int32, of ids' shape; 1 = the most likely token
+    top_logprobs: torch.Tensor | None     # (T, top), descending
+    top_ids: torch.Tensor | None          # (T, top) int32
+    entropy: torch.Tensor                 # (T,)
+    logsumexp: torch.Tensor               # (T,)
+
+
+LOGPROBS_MAX = 64
+LOGITS_TYPES = {torch.float32: 0, BF16: 1, torch.float16: 2}
+
+
+def _need_ids(ids, rows: int):
+    """Given tokens (rows,) or (rows, n <= 64), int32 or int64 -> n."""
+    if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int32, torch.int64):
+        raise MkError("ids: expected an int32 or int64 tensor")
+    if not ids.is_cuda:
+        raise MkError("ids: must be a GPU tensor (libmk has no CPU path)")
+    if ids.dim() not in (1, 2) or ids.shape[0] != rows:
+        raise MkError(f"ids: shape {tuple(ids.shape)}, expected ({rows},) or ({rows}, n)")
+    if not ids.is_contiguous():
+        raise MkError("ids: must be contiguous")
+    n = ids.shape[1] if ids.dim() == 2 else 1
+    if n > LOGPROBS_MAX:
+        raise MkError(f"ids: {n} given tokens a row, at most {LOGPROBS_MAX}")
+    return n
+
+
+def logprobs(logits: torch.Tensor, ids: torch.Tensor | None = None, top: int = 0) -> LogProbs:
+    """Log probabilities of rows of logits (T, V) f32 / bf16 / f16 in one pass (include/mk.h, mk_logprobs): of the
+    given tokens `ids` (T,) or (T, n) with their ranks, of the `top` most likely tokens, with entropy and logsumexp.
+
+    Equal logits rank by the lower index.  An id outside [0, V): -inf, rank -1.  A row of only -inf (everything
+    masked): log probabilities and logsumexp -inf, entropy 0.  A row with NaN or +inf: NaN, ranks and top_ids -1.
+    Rows may be strided (a slice of a padded vocabulary).  No gradient."""
+    lib = load()
+    _need_rows(logits, "logits", tuple(LOGITS_TYPES))
+    T, V = logits.shape
+    if V < 1:
+        raise MkError("logits: empty vocabulary")
+    top = int(top)
+    if not 0 <= top <= min(LOGPROBS_MAX, V):
+        raise MkError(f"top: {top}, expected 0 .. {min(LOGPROBS_MAX, V)}")
+    n = 0 if ids is None else _need_ids(ids, T)
+    _same_device(logits, ids=ids)
+    dev, f32, i32 = logits.device, torch.float32, torch.int32
+    with _on(logits):
+        lp = rk = tl = ti = None
+        if ids is not None:
+            lp, rk = torch.empty(ids.shape, dtype=f32, device=dev), torch.empty(ids.shape, dtype=i32, device=dev)
+        if top:
+            tl, ti = torch.empty((T, top), dtype=f32, device=dev), torch.empty((T, top), dtype=i32, device=dev)
+        ent, lse = torch.empty((T,), dtype=f32, device=dev), torch.empty((T,), dtype=f32, device=dev)
+        nbytes = int(lib.mk_logprobs_scratch_bytes(T, V, n, top))
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        check(lib.mk_logprobs(_ptr(logits), LOGITS_TYPES[logits.dtype], logits.stride(0), T, V, _ptr(ids),
+                              int(n > 0 and ids.dtype == torch.int64), n, top, _ptr(lp), _ptr(rk), _ptr(tl), _ptr(ti),
+                              _ptr(ent), _ptr(lse), _ptr(scratch), nbytes, _stream()), "mk_logprobs")
+    return LogProbs(lp, rk, tl, ti, ent, lse)
+
+
 def pack_weight(w: torch.Tensor, map_gu: bool = False, ic: int = 0, inter: int = 0) -> torch.Tensor:
     """(K, N) -> (N, K) repack (the layout mk_model_create builds); map_gu reorders gate/up columns."""
     lib = load()
@@ -170,4 +260,5 @@ def pack_weight(w: torch.Tensor, map_gu: bool = False, ic: int = 0, inter: int =
     return out
 
 
-__all__ = ["attn_prefill", "attn_scratch_bytes", "row_quant", "act_quant", "gemm", "lm_head", "pack_weight", "MkError", "_lib"]
+__all__ = ["attn_prefill", "attn_scratch_bytes", "row_quant", "act_quant", "gemm", "lm_head", "logprobs", "LogProbs",
+           "pack_weight", "MkError", "_lib"]
