@@ -19,7 +19,6 @@ namespace mk {
 
 namespace {
 
-constexpr int LP_WAVES = 4, LP_TH = 64 * LP_WAVES;
 constexpr int LP_E = 16;                 // values of a lane per tile
 constexpr int LP_TILE = 64 * LP_E;       // values of a wave per tile
 constexpr int LP_CAP = 128;              // list entries of a wave: the k <= 64 kept and one ballot's worth of new ones
@@ -28,16 +27,31 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ inline float neg_inf() { return -__builtin_inff(); }
 
-// Order of the alternatives: the larger value first, the lower index among equals.
-__device__ inline bool better(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
-
 __device__ inline void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
 
-// Running softmax statistics of one lane (or of a merged set).  m starts at the lowest finite value, so that a set
-// of only -inf has S = 0 and no infinity is subtracted from another.
+// Reductions over the wave, the result in every lane: within rows of 16 lanes by DPP (lane ^ 1, lane ^ 2, then mirrored
+// halves and rows, whose lanes hold equal values by then), across the four rows by two permutes.
+template <int CTRL>
+__device__ inline float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <class F>
+__device__ inline float wave_reduce(float v, F f) {
+  v = f(v, dpp<0xb1>(v));    // quad_perm [1, 0, 3, 2]
+  v = f(v, dpp<0x4e>(v));    // quad_perm [2, 3, 0, 1]
+  v = f(v, dpp<0x141>(v));   // row_half_mirror
+  v = f(v, dpp<0x140>(v));   // row_mirror
+  v = f(v, __shfl_xor(v, 16));
+  return f(v, __shfl_xor(v, 32));
+}
+__device__ inline float wave_max(float v) { return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ inline float wave_sum(float v) { return wave_reduce(v, [](float a, float b) { return a + b; }); }
+
+// Running softmax statistics.  m starts at the lowest finite value, so that a set of only -inf has S = 0 and no
+// infinity is subtracted from another.
 struct Stat {
   float m = NEG_MAX, s = 0.f, u = 0.f;
   // moves the reference maximum to mn >= m; the difference is kept finite (e^-1e4 is 0 anyway), 0 * -inf would be NaN
@@ -47,92 +61,90 @@ struct Stat {
     s *= f;
     m = mn;
   }
-  __device__ void merge(float m2, float s2, float u2) {
-    Stat o;
-    o.m = m2; o.s = s2; o.u = u2;
-    const float mn = fmaxf(m, m2);
-    raise(mn);
-    o.raise(mn);
-    s += o.s;
-    u += o.u;
+  // the wave's lanes as one
+  __device__ void reduce() {
+    raise(wave_max(m));
+    s = wave_sum(s);
+    u = wave_sum(u);
   }
 };
 
-// The k best (value, index) a wave has been offered, in the wave's LDS slice, and the threshold an entry has to beat:
-// no worse than the k-th best so far.
+// Values in sortable form: unsigned order is float order, -0 as +0 (NaN aside).
+__device__ inline uint32_t sort_key(float v) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return (int)b < 0 ? ~b : b | 0x80000000u;
+}
+__device__ inline float from_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+// An alternative as one number: the larger value first, the lower index among equals, is the larger entry.
+typedef unsigned long long u64;
+__device__ inline u64 entry(float v, int i) { return (u64)sort_key(v) << 32 | ~(uint32_t)i; }
+__device__ inline float entry_value(u64 e) { return from_key((uint32_t)(e >> 32)); }
+__device__ inline int entry_index(u64 e) { return (int)~(uint32_t)e; }
+
+// What a wave has kept of the values it was offered (a superset of its part of the k best), in the wave's LDS slice, and
+// the bound a new entry has to pass: above tv, or equal to it at an index below ti.
 struct TopList {
-  float* val;
-  int* idx;
+  u64* e;
   int k, cnt;
   float tv;
   int ti;
 
-  // index bound `end`: entries at end or beyond never enter (padding)
-  __device__ void init(float* v, int* i, int k_, int end) {
-    val = v; idx = i; k = k_; cnt = 0;
+  // indices at end or beyond never pass (padding)
+  __device__ void init(u64* e_, int k_, int end) {
+    e = e_; k = k_; cnt = 0;
     tv = neg_inf(); ti = end;
   }
-  __device__ bool passes(float v, int i) const { return better(v, i, tv, ti); }
-
-  // Keeps the k best of the list, in order, each entry's place the number of entries that beat it.
+  __device__ bool passes(float v, int i) const { return v > tv || (v == tv && i < ti); }
+  // at least k values of the row are known to be >= b
+  __device__ void bound(float b, int end) {
+    if (b > tv) {
+      tv = b;
+      ti = end;
+    }
+  }
+  // Keeps the k best: an entry's place is the number of entries above it.
   __device__ void prune() {
     const int lane = threadIdx.x & 63;
     wave_fence();
-    const bool h0 = lane < cnt, h1 = lane + 64 < cnt;
-    const float v0 = h0 ? val[lane] : 0.f, v1 = h1 ? val[lane + 64] : 0.f;
-    const int i0 = h0 ? idx[lane] : 0, i1 = h1 ? idx[lane + 64] : 0;
+    const u64 e0 = lane < cnt ? e[lane] : 0, e1 = lane + 64 < cnt ? e[lane + 64] : 0;
     int r0 = 0, r1 = 0;
+#pragma unroll 4
     for (int j = 0; j < cnt; ++j) {
-      const float v = val[j];
-      const int i = idx[j];
-      r0 += better(v, i, v0, i0);
-      r1 += better(v, i, v1, i1);
+      const u64 o = e[j];
+      r0 += o > e0;
+      r1 += o > e1;
     }
     wave_fence();
-    if (h0 && r0 < k) { val[r0] = v0; idx[r0] = i0; }
-    if (h1 && r1 < k) { val[r1] = v1; idx[r1] = i1; }
+    if (lane < cnt && r0 < k) e[r0] = e0;
+    if (lane + 64 < cnt && r1 < k) e[r1] = e1;
     wave_fence();
     if (cnt >= k) {
       cnt = k;
-      tv = val[k - 1];
-      ti = idx[k - 1];
+      tv = entry_value(e[k - 1]);
+      ti = entry_index(e[k - 1]);
     }
   }
-  // one value of every lane; the list has room for a whole ballot after a prune
-  __device__ void offer(float v, int i) {
-    unsigned long long mask = __ballot(passes(v, i));
-    if (!mask) return;
-    if (cnt + __popcll(mask) > LP_CAP) {
-      prune();
-      mask = __ballot(passes(v, i));
-      if (!mask) return;
-    }
-    if (passes(v, i)) {
-      const int at = cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-      val[at] = v;
-      idx[at] = i;
-    }
+  // Whether a lane with a value of v at index i0 or later may pass: the tie with the bound only below its index.
+  __device__ bool may_pass(float v, int i0) const { return i0 < ti ? v >= tv : v > tv; }
+  // one value of the lanes that have one; after a prune the list has room for a whole ballot
+  __device__ void offer(bool have, float v, int i) {
+    if (cnt > LP_CAP - 64) prune();
+    const bool in = have && passes(v, i);
+    const u64 mask = __ballot(in);
+    if (in)
+      e[cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = entry(v, i);
     cnt += __popcll(mask);
   }
 };
 
-// Values in sortable form: unsigned order is float order (NaN aside; -0 just below +0, which only loosens a bound).
-__device__ inline uint32_t sort_key(float v) {
-  const uint32_t b = __float_as_uint(v);
-  return (int)b < 0 ? ~b : b | 0x80000000u;
-}
-__device__ inline float from_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
-
 // A value that at least k of the wave's 64 lanes reach with v (k <= 64): the k-th largest lane value cut to its upper
-// 16 key bits, by bisection on ballots.  At least k values of a tile are at least this large when v is the lanes' maxima.
+// 16 key bits, by bisection on ballots.
 __device__ inline float kth_bound(float v, int k) {
   const uint32_t key = sort_key(v);
   uint32_t t = 0;
-#pragma unroll
-  for (int b = 31; b >= 16; --b) {
-    const uint32_t c = t | (1u << b);
-    if (__popcll(__ballot(key >= c)) >= k) t = c;
-  }
+#pragma unroll 4
+  for (uint32_t b = 1u << 31; b >= 1u << 16; b >>= 1)
+    if (__popcll(__ballot(key >= (t | b))) >= k) t |= b;
   return t < sort_key(neg_inf()) ? neg_inf() : from_key(t);
 }
 
@@ -169,92 +181,106 @@ struct Load<_Float16> {
   }
 };
 
-// Workspace entry of one (row, split): m, s, u, unused; n_ids counts; k values; k indices.
-__host__ __device__ inline size_t part_floats(int n_ids, int k) { return 4 + (size_t)n_ids + 2 * (size_t)k; }
+// Workspace of one (row, split): m, s, u, unused; of each given token the count of values above it and, from the split
+// that holds it, its value; the list of k entries, 8-byte aligned.
+__host__ __device__ inline size_t part_floats(int n_ids, int k) { return 4 + 2 * (size_t)n_ids + 2 * (size_t)k; }
 
+template <int WAVES>
 struct RowShared {
-  float val[LP_WAVES][LP_CAP];
-  int idx[LP_WAVES][LP_CAP];
-  float m[LP_WAVES], s[LP_WAVES], u[LP_WAVES];
-  int cnt[LP_WAVES];
-  float idv[LP_MAX_IDS];
-  int idn[LP_MAX_IDS];
-  int rank[LP_WAVES][LP_MAX_IDS];
+  u64 list[WAVES][LP_CAP];   // by wave
+  u64 all[WAVES * 64];       // what is left of them at the end, in any order
+  float m[WAVES], s[WAVES], u[WAVES];
+  int n;                     // entries of all
+  float gmax[64];            // largest value seen by each of 64 groups of lanes
+  int rank[WAVES][LP_MAX_IDS];
+};
+
+// The waves' statistics as one, in every thread.
+template <int WAVES>
+__device__ inline Stat merge_stats(const RowShared<WAVES>& sh) {
+  Stat st;
+#pragma unroll
+  for (int o = 0; o < WAVES; ++o) st.m = fmaxf(st.m, sh.m[o]);
+#pragma unroll
+  for (int o = 0; o < WAVES; ++o) {
+    Stat x;
+    x.m = sh.m[o]; x.s = sh.s[o]; x.u = sh.u[o];
+    x.raise(st.m);
+    st.s += x.s;
+    st.u += x.u;
+  }
+  return st;
+}
+
+// The wave's list, at most 64 entries of it, into sh.all.
+template <int WAVES>
+__device__ inline void give_list(RowShared<WAVES>& sh, TopList& top) {
+  const int lane = threadIdx.x & 63;
+  if (top.cnt > 64) top.prune();
+  int base = 0;
+  if (lane == 0) base = atomicAdd(&sh.n, top.cnt);
+  base = __builtin_amdgcn_readfirstlane(base);
+  wave_fence();
+  if (lane < top.cnt) sh.all[base + lane] = top.e[lane];
+}
+
+// The k best of sh.all: every entry counts the entries above it and, if fewer than k, takes that place, whatever the
+// order they lie in.  put(place, entry)
+template <int WAVES, class F>
+__device__ inline void best_of_all(const RowShared<WAVES>& sh, int k, F put) {
+  const int n = sh.n;
+  for (int t = threadIdx.x; t < n; t += 64 * WAVES) {
+    const u64 e = sh.all[t];
+    int r = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) r += sh.all[j] > e;
+    if (r < k) put(r, e);
+  }
+}
+
+// The row's outputs: st its statistics, lane j of wave 0 given token j (id < 0: outside the vocabulary) with its
+// value and the count of values above it.
+struct RowOut {
+  bool nan, empty;
+  Stat st;
+  float ls;
+  __device__ RowOut(const Stat& s) : st(s) {
+    nan = !(s.s == s.s);     // an infinite logit makes s NaN as well
+    empty = s.s == 0.f;
+    ls = logf(s.s);
+  }
+  __device__ float lp(float v) const {
+    return nan ? __builtin_nanf("") : empty ? neg_inf() : (v - st.m) - ls;
+  }
+  __device__ void stats(const LogprobArgs& a, int row) const {
+    a.lse[row] = nan ? __builtin_nanf("") : empty ? neg_inf() : st.m + ls;
+    a.entropy[row] = nan ? __builtin_nanf("") : empty ? 0.f : ls - st.u / st.s;
+  }
+  __device__ void token(const LogprobArgs& a, int row, int j, bool in, float v, int above) const {
+    const size_t o = (size_t)row * a.n_ids + j;
+    a.token_lp[o] = nan || in ? lp(v) : neg_inf();
+    a.ranks[o] = nan || !in ? -1 : 1 + above;
+  }
+  __device__ void top(const LogprobArgs& a, int row, int place, u64 e) const {
+    const size_t o = (size_t)row * a.top + place;
+    a.top_lp[o] = lp(entry_value(e));
+    a.top_ids[o] = nan ? -1 : entry_index(e);
+  }
 };
 
 __device__ inline long long id_at(const LogprobArgs& a, size_t i) {
   return a.ids64 ? static_cast<const long long*>(a.ids)[i] : static_cast<const int*>(a.ids)[i];
 }
 
-// The row's given tokens: index (-1 outside the vocabulary) and value, into LDS by the whole workgroup.
-template <typename T>
-__device__ inline void load_ids(const LogprobArgs& a, int row, const T* x, RowShared& sh) {
-  for (int j = threadIdx.x; j < a.n_ids; j += LP_TH) {
-    const long long id = id_at(a, (size_t)row * a.n_ids + j);
-    const bool in = id >= 0 && id < a.V;
-    sh.idn[j] = in ? (int)id : -1;
-    sh.idv[j] = in ? Load<T>::f(x[id]) : __builtin_inff();
-  }
-}
-
-// Merged statistics st (all threads), ranks' counts in sh.rank[0], the sorted list of cnt entries in lv / li (LDS)
-// -> the row's outputs.
-__device__ inline void write_row(const LogprobArgs& a, int row, const Stat& st, const RowShared& sh, const float* lv,
-                                 const int* li) {
-  const bool nan = !(st.s == st.s), empty = st.s == 0.f;   // an infinite logit makes s NaN as well
-  const float q = __builtin_nanf(""), ls = logf(st.s);
-  if (threadIdx.x == 0) {
-    a.lse[row] = nan ? q : empty ? neg_inf() : st.m + ls;
-    a.entropy[row] = nan ? q : empty ? 0.f : ls - st.u / st.s;
-  }
-  for (int j = threadIdx.x; j < a.n_ids; j += LP_TH) {
-    const size_t o = (size_t)row * a.n_ids + j;
-    const bool in = sh.idn[j] >= 0;
-    a.token_lp[o] = nan ? q : empty || !in ? neg_inf() : (sh.idv[j] - st.m) - ls;
-    a.ranks[o] = nan || !in ? -1 : 1 + sh.rank[0][j];
-  }
-  for (int j = threadIdx.x; j < a.top; j += LP_TH) {
-    const size_t o = (size_t)row * a.top + j;
-    a.top_lp[o] = nan ? q : empty ? neg_inf() : (lv[j] - st.m) - ls;
-    a.top_ids[o] = nan ? -1 : li[j];
-  }
-}
-
-// Merges the waves' sorted lists (counts in sh.cnt): entry e of wave w goes to its place among all.  The places below k
-// are written to ov / oi, which must not be the lists.
-__device__ inline void merge_lists(const RowShared& sh, int k, float* ov, int* oi) {
-  const int w = threadIdx.x >> 6, e = threadIdx.x & 63;
-  if (e >= min(sh.cnt[w], k)) return;
-  const float v = sh.val[w][e];
-  const int i = sh.idx[w][e];
-  int place = e;
-#pragma unroll
-  for (int o = 0; o < LP_WAVES; ++o) {
-    if (o == w) continue;
-    int lo = 0, hi = min(sh.cnt[o], k);
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (better(sh.val[o][mid], sh.idx[o][mid], v, i)) lo = mid + 1;
-      else hi = mid;
-    }
-    place += lo;
-  }
-  if (place < k) {
-    ov[place] = v;
-    oi[place] = i;
-  }
-}
-
-// One (row, split): values [split * chunk, min(V, + chunk)) of the row, chunk a multiple of LP_TILE.  The waves take
-// its tiles in turn, so that a wave sees its values in index order tile by tile.
-template <typename T, bool SPLIT>
-__global__ __launch_bounds__(LP_TH, 6) void logprob_rows_kernel(LogprobArgs a, int splits, int chunk, float* part) {
+// One (row, split): values [split * chunk, min(V, + chunk)) of the row, chunk a multiple of LP_TILE.  The waves take its
+// tiles in turn.  Given token j belongs to lane j of every wave.
+template <typename T, int WAVES, bool SPLIT>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 6) void logprob_rows_kernel(LogprobArgs a, int splits, int chunk,
+                                                                                       float* part) {
   using L = Load<T>;
-  constexpr int VEC = L::VEC, NV = LP_E / VEC;
-  __shared__ RowShared sh;
-  __shared__ float ov[LP_MAX_TOP];
-  __shared__ int oi[LP_MAX_TOP];
-  const int row = blockIdx.x / splits, split = blockIdx.x - row * splits;
+  constexpr int VEC = L::VEC, NV = LP_E / VEC, TH = 64 * WAVES;
+  __shared__ RowShared<WAVES> sh;
+  const int row = SPLIT ? blockIdx.x / splits : blockIdx.x, split = SPLIT ? blockIdx.x - row * splits : 0;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T* x = static_cast<const T*>(a.x) + (size_t)row * a.ldx;
@@ -269,26 +295,44 @@ __global__ __launch_bounds__(LP_TH, 6) void logprob_rows_kernel(LogprobArgs a, i
   };
   int t0 = c0 + w * LP_TILE;
   if (t0 + LP_TILE <= c1) load(t0);
-  load_ids<T>(a, row, x, sh);
-  for (int j = lane; j < a.n_ids; j += 64) sh.rank[w][j] = 0;
-  __syncthreads();
+  int id = -1, above = 0;
+  float iv = __builtin_inff();
+  if (lane < a.n_ids) {
+    const long long i = id_at(a, (size_t)row * a.n_ids + lane);
+    if (i >= 0 && i < a.V) {
+      id = (int)i;
+      iv = L::f(x[id]);
+    }
+  }
+  if (threadIdx.x == 0) sh.n = 0;          // read after the loop's barrier
+  float lmax = neg_inf();
+  auto publish = [&] {
+    float g = lmax;
+    g = fmaxf(g, dpp<0xb1>(g));
+    g = fmaxf(g, dpp<0x4e>(g));
+    if constexpr (WAVES >= 8) g = fmaxf(g, dpp<0x141>(g));
+    if constexpr (WAVES >= 16) g = fmaxf(g, dpp<0x140>(g));
+    constexpr int LANES = WAVES;           // of a group
+    static_assert(LANES == 4 || LANES == 8 || LANES == 16, "groups are quads, half rows or rows");
+    if (lane % LANES == 0) *const_cast<volatile float*>(&sh.gmax[threadIdx.x / LANES]) = g;
+  };
 
   Stat st;
   TopList top;
-  top.init(sh.val[w], sh.idx[w], a.top, c1);
-  for (; t0 < c1; t0 += LP_WAVES * LP_TILE) {
+  top.init(sh.list[w], a.top, c1);
+  for (bool first = true; first || t0 < c1; first = false, t0 += WAVES * LP_TILE) {
     float v[LP_E];
     if (t0 + LP_TILE <= c1) {
 #pragma unroll
       for (int q = 0; q < NV; ++q) L::unpack(raw[q], v + q * VEC);
-    } else {
+    } else {   // the last tile, or a first one of nothing
 #pragma unroll
       for (int e = 0; e < LP_E; ++e) {
         const int i = at(t0, e);
         v[e] = i < c1 ? L::f(x[i]) : neg_inf();
       }
     }
-    const int tn = t0 + LP_WAVES * LP_TILE;
+    const int tn = t0 + WAVES * LP_TILE;
     if (tn + LP_TILE <= c1) load(tn);
 
     float tm = v[0];
@@ -307,64 +351,73 @@ __global__ __launch_bounds__(LP_TH, 6) void logprob_rows_kernel(LogprobArgs a, i
     st.u += u;
 
     for (int j = 0; j < a.n_ids; ++j) {
-      const float iv = sh.idv[j];
-      const int id = sh.idn[j];
+      const float jv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(iv), j));
+      const int ji = __builtin_amdgcn_readlane(id, j);
       int n = 0;
-      if (t0 + LP_TILE <= id) {            // every value here has a lower index
+      if (t0 + LP_TILE <= ji) {            // every value here has a lower index
 #pragma unroll
-        for (int e = 0; e < LP_E; ++e) n += __popcll(__ballot(v[e] >= iv));
-      } else if (t0 > id) {
+        for (int e = 0; e < LP_E; ++e) n += __popcll(__ballot(v[e] >= jv));
+      } else if (t0 > ji) {
 #pragma unroll
-        for (int e = 0; e < LP_E; ++e) n += __popcll(__ballot(v[e] > iv));
+        for (int e = 0; e < LP_E; ++e) n += __popcll(__ballot(v[e] > jv));
       } else {
 #pragma unroll
-        for (int e = 0; e < LP_E; ++e) n += __popcll(__ballot(better(v[e], at(t0, e), iv, id)));
+        for (int e = 0; e < LP_E; ++e) n += __popcll(__ballot(v[e] > jv || (v[e] == jv && at(t0, e) < ji)));
       }
-      if (lane == 0) sh.rank[w][j] += n;
+      above += lane == j ? n : 0;
     }
 
-    if (a.top && __ballot(tm >= top.tv)) {
-      if (top.cnt == 0) {                  // nothing known yet: a bound from the lanes' maxima
-        const float b = kth_bound(tm, top.k);
-        if (b > top.tv) {
-          top.tv = b;
-          top.ti = c1;
+    if (a.top) {
+      // Lower bounds of the k-th best, so that few values of a row are ever listed.  64 groups of lanes (a row of 16 of
+      // 16 waves, a quad of 4 waves) publish the largest value each has seen; the k-th largest of those is reached by k
+      // values: of 16384 random ones about 24 reach the bound for k = 20.  A wave takes a new bound only where a value of
+      // its tile passes the last one.  Other waves' entries may be older: lower, still bounds.
+      lmax = fmaxf(lmax, tm);
+      if (first) {
+        top.bound(kth_bound(tm, a.top), c1);   // where less than k groups have a value
+        publish();
+        __syncthreads();
+      }
+      if (__ballot(top.may_pass(tm, t0))) {
+        if (!first) publish();
+        top.bound(kth_bound(*const_cast<volatile float*>(&sh.gmax[lane]), a.top), c1);
+        uint32_t some = 0;                 // the lane's values that may pass; few, and read again: v has no index
+#pragma unroll
+        for (int e = 0; e < LP_E; ++e) some |= (uint32_t)top.may_pass(v[e], t0) << e;
+        while (__ballot(some)) {
+          const int i = at(t0, __builtin_ctz(some | 1u << LP_E));
+          const bool have = some && i < c1;
+          top.offer(have, have ? L::f(x[i]) : 0.f, i);
+          some &= some - 1;
         }
       }
-#pragma unroll
-      for (int e = 0; e < LP_E; ++e) top.offer(v[e], at(t0, e));
-      if (top.cnt > min(top.k + 32, 2 * top.k)) top.prune();
     }
   }
 
-  // the lanes' statistics, then the waves'
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) st.merge(__shfl_xor(st.m, o), __shfl_xor(st.s, o), __shfl_xor(st.u, o));
-  if (a.top) top.prune();
+  st.reduce();
   if (lane == 0) {
     sh.m[w] = st.m;
     sh.s[w] = st.s;
     sh.u[w] = st.u;
-    sh.cnt[w] = top.cnt;
   }
-  for (int j = threadIdx.x; j < a.top; j += LP_TH) {
-    ov[j] = neg_inf();
-    oi[j] = 0x7fffffff;
-  }
+  if (a.top) give_list(sh, top);
+  if (lane < a.n_ids) sh.rank[w][lane] = above;
   __syncthreads();
-  Stat all;
+  if (w == 0 && lane < a.n_ids) {
+    above = 0;
 #pragma unroll
-  for (int o = 0; o < LP_WAVES; ++o) all.merge(sh.m[o], sh.s[o], sh.u[o]);
-  for (int j = threadIdx.x; j < a.n_ids; j += LP_TH) {
-    int n = 0;
-#pragma unroll
-    for (int o = 0; o < LP_WAVES; ++o) n += sh.rank[o][j];
-    sh.rank[0][j] = n;
+    for (int o = 0; o < WAVES; ++o) above += sh.rank[o][lane];
   }
-  if (a.top) merge_lists(sh, a.top, ov, oi);
-  __syncthreads();
+  const Stat all = merge_stats(sh);
   if constexpr (!SPLIT) {
-    write_row(a, row, all, sh, ov, oi);
+    const RowOut out(all);
+    if (threadIdx.x == 0) out.stats(a, row);
+    if (w == 0 && lane < a.n_ids) out.token(a, row, lane, id >= 0, iv, above);
+    if (out.nan) {
+      for (int j = threadIdx.x; j < a.top; j += TH) out.top(a, row, j, 0);
+    } else if (a.top) {
+      best_of_all(sh, a.top, [&](int place, u64 e) { out.top(a, row, place, e); });
+    }
   } else {
     float* p = part + (size_t)blockIdx.x * part_floats(a.n_ids, a.top);
     if (threadIdx.x == 0) {
@@ -372,89 +425,95 @@ __global__ __launch_bounds__(LP_TH, 6) void logprob_rows_kernel(LogprobArgs a, i
       p[1] = all.s;
       p[2] = all.u;
     }
-    for (int j = threadIdx.x; j < a.n_ids; j += LP_TH) reinterpret_cast<int*>(p)[4 + j] = sh.rank[0][j];
-    float* pv = p + 4 + a.n_ids;
-    for (int j = threadIdx.x; j < a.top; j += LP_TH) {
-      pv[j] = ov[j];
-      reinterpret_cast<int*>(pv)[a.top + j] = oi[j];
+    if (w == 0 && lane < a.n_ids) {
+      reinterpret_cast<int*>(p)[4 + 2 * lane] = above;
+      p[5 + 2 * lane] = iv;
     }
+    u64* pe = reinterpret_cast<u64*>(p + 4 + 2 * a.n_ids);
+    if (a.top && threadIdx.x < a.top && threadIdx.x >= sh.n) pe[threadIdx.x] = 0;   // below every value's entry
+    if (a.top) best_of_all(sh, a.top, [&](int place, u64 e) { pe[place] = e; });
   }
 }
 
-// One row from its splits' entries, in a fixed order.
-template <typename T>
-__global__ __launch_bounds__(LP_TH) void logprob_merge_kernel(LogprobArgs a, int splits, const float* part) {
-  __shared__ RowShared sh;
-  __shared__ float ov[LP_MAX_TOP];
-  __shared__ int oi[LP_MAX_TOP];
+// One row from its splits' workspace entries, in a fixed order.  Four waves: the splits are few.
+__global__ __launch_bounds__(256) void logprob_merge_kernel(LogprobArgs a, int splits, const float* part) {
+  __shared__ RowShared<4> sh;
   const int row = blockIdx.x, lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const size_t pf = part_floats(a.n_ids, a.top);
   const float* p = part + (size_t)row * splits * pf;
-  load_ids<T>(a, row, static_cast<const T*>(a.x) + (size_t)row * a.ldx, sh);
 
   Stat st;
-  for (int i = threadIdx.x; i < splits; i += LP_TH) st.merge(p[i * pf], p[i * pf + 1], p[i * pf + 2]);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) st.merge(__shfl_xor(st.m, o), __shfl_xor(st.s, o), __shfl_xor(st.u, o));
+  for (int i = threadIdx.x; i < splits; i += 256) {
+    Stat x;
+    x.m = p[i * pf]; x.s = p[i * pf + 1]; x.u = p[i * pf + 2];
+    const float mn = fmaxf(st.m, x.m);
+    st.raise(mn);
+    x.raise(mn);
+    st.s += x.s;
+    st.u += x.u;
+  }
+  int above = 0;
+  bool in = false;
+  float iv = 0.f;
+  if (w == 0 && lane < a.n_ids) {
+    const long long i = id_at(a, (size_t)row * a.n_ids + lane);
+    in = i >= 0 && i < a.V;
+    iv = p[5 + 2 * lane];
+    for (int q = 0; q < splits; ++q) above += reinterpret_cast<const int*>(p + q * pf)[4 + 2 * lane];
+  }
+  if (threadIdx.x == 0) sh.n = 0;
+  __syncthreads();
+  TopList top;
+  top.init(sh.list[w], a.top, a.V);
+  if (a.top) {
+    const int k = a.top, n = splits * k;
+    auto get = [&](int i) {
+      const int s = i / k, j = i - s * k;
+      return reinterpret_cast<const u64*>(p + s * pf + 4 + 2 * a.n_ids)[j];
+    };
+    for (int i = w * 64; i < n; i += 256) {
+      const u64 e = i + lane < n ? get(i + lane) : 0;
+      const float v = e ? entry_value(e) : neg_inf();
+      const int at = e ? entry_index(e) : a.V;
+      if (i == w * 64) top.bound(kth_bound(v, k), a.V);
+      top.offer(e != 0, v, at);
+    }
+    give_list(sh, top);
+  }
+  st.reduce();
   if (lane == 0) {
     sh.m[w] = st.m;
     sh.s[w] = st.s;
     sh.u[w] = st.u;
   }
-  for (int j = threadIdx.x; j < a.n_ids; j += LP_TH) {
-    int n = 0;
-    for (int i = 0; i < splits; ++i) n += reinterpret_cast<const int*>(p + i * pf)[4 + j];
-    sh.rank[0][j] = n;
-  }
-  if (a.top) {
-    const int k = a.top, n = splits * k;
-    TopList top;
-    top.init(sh.val[w], sh.idx[w], k, a.V);
-    for (int i = w * 64; i < n; i += LP_TH) {
-      const int e = i + lane, s = min(e, n - 1) / k, j = min(e, n - 1) - s * k;
-      const float* pv = p + s * pf + 4 + a.n_ids;
-      // lanes past the entries hold what the splits' own padding is: -inf under an index that no bound admits
-      const float v = e < n ? pv[j] : neg_inf();
-      const int id = e < n ? reinterpret_cast<const int*>(pv)[k + j] : 0x7fffffff;
-      if (top.cnt == 0) {
-        const float b = kth_bound(v, k);
-        if (b > top.tv) {
-          top.tv = b;
-          top.ti = a.V;
-        }
-      }
-      top.offer(v, id);
-      if (top.cnt > min(k + 32, 2 * k)) top.prune();
-    }
-    top.prune();
-    if (lane == 0) sh.cnt[w] = top.cnt;
-    for (int j = threadIdx.x; j < k; j += LP_TH) {
-      ov[j] = neg_inf();
-      oi[j] = 0x7fffffff;
-    }
-  }
   __syncthreads();
-  Stat all;
-#pragma unroll
-  for (int o = 0; o < LP_WAVES; ++o) all.merge(sh.m[o], sh.s[o], sh.u[o]);
-  if (a.top) merge_lists(sh, a.top, ov, oi);
-  __syncthreads();
-  write_row(a, row, all, sh, ov, oi);
+  const RowOut out(merge_stats(sh));
+  if (threadIdx.x == 0) out.stats(a, row);
+  if (w == 0 && lane < a.n_ids) out.token(a, row, lane, in, iv, above);
+  if (out.nan) {
+    for (int j = threadIdx.x; j < a.top; j += 256) out.top(a, row, j, 0);
+  } else if (a.top) {
+    best_of_all(sh, a.top, [&](int place, u64 e) { out.top(a, row, place, e); });
+  }
 }
 
 template <typename T>
 int launch_t(const LogprobArgs& a, void* ws, hipStream_t st) {
-  const int splits = logprob_splits(a.T, a.V);
+  const LogprobPlan pl = logprob_plan(a.T, a.V);
   const int tiles = (a.V + LP_TILE - 1) / LP_TILE;
-  const int chunk = (tiles + splits - 1) / splits * LP_TILE;
+  const int chunk = (tiles + pl.splits - 1) / pl.splits * LP_TILE;
   float* part = static_cast<float*>(ws);
-  const dim3 block(LP_TH);
-  if (splits == 1) {
-    hipLaunchKernelGGL((logprob_rows_kernel<T, false>), dim3(a.T), block, 0, st, a, 1, chunk, nullptr);
+  if (pl.splits > 1) {
+    hipLaunchKernelGGL((logprob_rows_kernel<T, 16, true>), dim3((unsigned)(a.T * pl.splits)), dim3(1024), 0, st, a, pl.splits,
+                       chunk, part);
+    hipLaunchKernelGGL(logprob_merge_kernel, dim3(a.T), dim3(256), 0, st, a, pl.splits, part);
+  } else if (pl.waves == 8) {
+    hipLaunchKernelGGL((logprob_rows_kernel<T, 8, false>), dim3(a.T), dim3(512), 0, st, a, 1, chunk, nullptr);
+  } else if (pl.waves == 16) {
+    hipLaunchKernelGGL((logprob_rows_kernel<T, 16, false>), dim3(a.T), dim3(1024), 0, st, a, 1, chunk, nullptr);
   } else {
-    hipLaunchKernelGGL((logprob_rows_kernel<T, true>), dim3((unsigned)((size_t)a.T * splits)), block, 0, st, a, splits, chunk, part);
-    hipLaunchKernelGGL((logprob_merge_kernel<T>), dim3(a.T), block, 0, st, a, splits, part);
+    hipLaunchKernelGGL((logprob_rows_kernel<T, 4, false>), dim3(a.T), dim3(256), 0, st, a, 1, chunk, nullptr);
   }
   MK_HIP_CHECK(hipGetLastError());
   return MK_OK;
@@ -463,7 +522,7 @@ int launch_t(const LogprobArgs& a, void* ws, hipStream_t st) {
 }  // namespace
 
 size_t logprob_scratch_bytes(int T, int V, int n_ids, int top) {
-  const int splits = logprob_splits(T, V);
+  const int splits = logprob_plan(T, V).splits;
   return splits == 1 ? 0 : (size_t)T * splits * part_floats(n_ids, top) * sizeof(float);
 }
 

@@ -138,12 +138,20 @@ inline bool lm_head_skinny(int rows, int V, int K) {
   return K > 1536 && (rows == 1 || (rows == 2 && V >= 3 * 128 * 256));
 }
 
-// Workgroups that share a row of the log-probability pass: one per row once the rows fill the 256 CUs, else enough for
-// four a CU, each with a whole 1024-value tile for each of its 4 waves.
-inline int logprob_splits(int T, int V) {
-  const int most = (V + 4095) / 4096, want = (1024 + T - 1) / T;
-  if (T >= 256 || most <= 1) return 1;
-  return want < most ? want : most;
+// How the log-probability pass divides (T, V): workgroups a row, waves a workgroup (1024 values a wave and step).
+// Many rows: small workgroups, several a CU, whose row ends overlap (us, bf16 V = 130560: 3000 rows with 4 waves 195, 8
+// 203, 16 288; V = 8000, 4096 rows 41, 58, 122).  Rows for one or two workgroups a CU: more waves each (bf16 V = 130560,
+// 500 rows 52, 40, 46; 700 rows 60, 52, 65; f32 1000 rows 107, 114, 114; 200 rows 72, 48, 35).  Few long rows are split,
+// as the exponentials of a 130560-value row alone take one CU 12 us; that costs a second launch (f32 V = 130560, one
+// then split: 1 row 24.0, 13.1, 33 rows 36.3, 24.8, 65 rows 29.7, 22.6, 200 rows in two 34.7, 46.5; 8 rows of 65536
+// 17.3, 13.5).
+struct LogprobPlan { int splits, waves; };
+inline LogprobPlan logprob_plan(int T, int V) {
+  if (T > 896) return {1, 4};
+  if (T > 256) return {1, 8};
+  const int most = ((V + 1023) / 1024 + 15) / 16, room = T > 0 ? 256 / T : 1;
+  if (most <= 2 || room <= 1) return {1, 16};
+  return {most < room ? most : room, 16};
 }
 
 }  // namespace mk

@@ -46,8 +46,8 @@ def test_logprobs_refusals(kw, code, msg):
 
 def test_logprobs_scratch():
     f = _lib.load().mk_logprobs_scratch_bytes
-    assert f(256, 130560, 1, 20) == 0 and f(4, 4096, 1, 20) == 0     # one workgroup a row
-    assert f(1, 130560, 1, 20) == 32 * (4 + 1 + 40) * 4              # 32 of 4096 values
+    assert f(2000, 130560, 1, 20) == 0 and f(4, 32768, 1, 20) == 0   # one workgroup a row
+    assert f(1, 130560, 1, 20) == 8 * (4 + 2 + 40) * 4               # 8 of 16384 values
     assert f(0, 130560, 1, 20) == 0 and f(1, 0, 1, 1) == 0
 
 
