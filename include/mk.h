@@ -273,6 +273,24 @@ int mk_logprobs(const void* logits, int type, size_t ld, int T, int V, const voi
                 float* token_lp, int32_t* ranks, float* top_lp, int32_t* top_ids, float* entropy, float* lse,
                 void* scratch, size_t scratch_bytes, void* stream);
 
+/* 4-bit weights with group scales (no counterpart in the reference).  W (N, K) bf16, row stride ldw elements; along K
+ * each row is cut into groups of `group` (32, 64 or 128) values, the last one shorter.  Of a group:
+ *   s = bf16(amax / 7), 0 where amax / 7 < 2^-126, NaN where a value is not finite;
+ *   c = clip(round_half_even(w / s), -7, 7), 0 where s = 0;   W ~ c s
+ * mk_w4_bytes: sizes of the two buffers, codes (whole blocks of 16 rows x 128 values) and scales, 32-byte aligned each.
+ * mk_w4_dequantize: out (N, K) = c s, bf16 (rounded once) or f32 (exact), row stride ldo elements.
+ * mk_gemm_w4: out (M, N) = x (M, K) (c s)^T, x bf16 at row stride ldx, f32 accumulation, out bf16 or f32 at row stride
+ *   ldo; made for few rows (the weights are read once per 64 of them).  |x| up to 2^110: the codes are multiplied with an
+ *   offset that is taken off again.  A row of x with an infinity or a NaN, and a weight row with a NaN scale, give NaN.
+ * N, K >= 1, M >= 0; any alignment and stride of whole elements for W, x and out.  Results do not depend on timing; a
+ * row's result does not depend on the other rows. */
+int mk_w4_bytes(int N, int K, int group, size_t* codes, size_t* scales);
+int mk_w4_quantize(const void* w, size_t ldw, int N, int K, int group, void* codes, void* scales, void* stream);
+int mk_w4_dequantize(const void* codes, const void* scales, int N, int K, int group, void* out, int out_f32, size_t ldo,
+                     void* stream);
+int mk_gemm_w4(const void* x, size_t ldx, const void* codes, const void* scales, int M, int N, int K, int group, void* out,
+               int out_f32, size_t ldo, void* stream);
+
 /* Weight preparation on the GPU: the per-parameter work of prepare_mk_weights (mk_weights.py:113-123,
  * :229-252), bit-identical to the CPU restatement; the small FP32 calibration forward stays on the host.
  * w is an HF linear weight (n_out, n_in) bf16 and W = w^T * fold its (in, out) f32 view (fold = 1/sqrt(hd)

@@ -361,6 +361,72 @@ int mk_logprobs(const void* logits, int type, size_t ld, int T, int V, const voi
   MK_TRY(mk::launch_logprobs(a, scratch, static_cast<hipStream_t>(stream)));
 }
 
+namespace {
+bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int w4_validate(const char* what, int N, int K, int group) {
+  const std::string w(what);
+  MK_REQUIRE(group == 32 || group == 64 || group == 128, w + ": group must be 32, 64 or 128");
+  MK_REQUIRE(N >= 1 && K >= 1, w + ": empty weight");
+  MK_REQUIRE(N <= (1 << 30) && K <= (1 << 30) && (long)((N + 15) / 16) * ((K + 127) / 128) < (1L << 32),
+             w + ": weight too large");
+  return MK_OK;
+}
+
+int w4_buffers(const char* what, const void* codes, const void* scales) {
+  const std::string w(what);
+  MK_REQUIRE(codes && scales, w + ": null weight");
+  MK_REQUIRE(aligned_to(codes, 32) && aligned_to(scales, 32), w + ": codes and scales must be 32-byte aligned");
+  return MK_OK;
+}
+}  // namespace
+
+int mk_w4_bytes(int N, int K, int group, size_t* codes, size_t* scales) {
+  int rc = w4_validate("w4_bytes", N, K, group);
+  if (rc) return rc;
+  MK_REQUIRE(codes && scales, "w4_bytes: null output");
+  const size_t blocks = (size_t)((N + 15) / 16) * ((K + 127) / 128);
+  *codes = blocks * 1024;
+  *scales = blocks * 16 * (128 / group) * 2;
+  return MK_OK;
+}
+
+int mk_w4_quantize(const void* w, size_t ldw, int N, int K, int group, void* codes, void* scales, void* stream) {
+  int rc = w4_validate("w4_quantize", N, K, group);
+  if (!rc) rc = w4_buffers("w4_quantize", codes, scales);
+  if (rc) return rc;
+  MK_REQUIRE(w && aligned_to(w, 2), "w4_quantize: null or misaligned weight");
+  MK_REQUIRE(ldw >= (size_t)K || N == 1, "w4_quantize: row stride below K");
+  MK_TRY(mk::launch_w4_quantize(static_cast<const uint16_t*>(w), ldw, N, K, group, static_cast<uint8_t*>(codes),
+                                static_cast<uint16_t*>(scales), static_cast<hipStream_t>(stream)));
+}
+
+int mk_w4_dequantize(const void* codes, const void* scales, int N, int K, int group, void* out, int out_f32, size_t ldo,
+                     void* stream) {
+  int rc = w4_validate("w4_dequantize", N, K, group);
+  if (!rc) rc = w4_buffers("w4_dequantize", codes, scales);
+  if (rc) return rc;
+  MK_REQUIRE(out && aligned_to(out, out_f32 ? 4 : 2), "w4_dequantize: null or misaligned output");
+  MK_REQUIRE(ldo >= (size_t)K || N == 1, "w4_dequantize: row stride below K");
+  MK_TRY(mk::launch_w4_dequantize(static_cast<const uint8_t*>(codes), static_cast<const uint16_t*>(scales), N, K, group, out,
+                                  out_f32 != 0, ldo, static_cast<hipStream_t>(stream)));
+}
+
+int mk_gemm_w4(const void* x, size_t ldx, const void* codes, const void* scales, int M, int N, int K, int group, void* out,
+               int out_f32, size_t ldo, void* stream) {
+  int rc = w4_validate("gemm_w4", N, K, group);
+  if (rc) return rc;
+  MK_REQUIRE(M >= 0, "gemm_w4: negative M");
+  if (M == 0) return MK_OK;
+  rc = w4_buffers("gemm_w4", codes, scales);
+  if (rc) return rc;
+  MK_REQUIRE(x && out && aligned_to(x, 2) && aligned_to(out, out_f32 ? 4 : 2), "gemm_w4: null or misaligned x or out");
+  MK_REQUIRE(M == 1 || (ldx >= (size_t)K && ldo >= (size_t)N), "gemm_w4: row stride below the row");
+  const mk::W4GemmArgs a{static_cast<const uint16_t*>(x), ldx, static_cast<const uint8_t*>(codes),
+                         static_cast<const uint16_t*>(scales), out, ldo, out_f32 != 0, M, N, K, group};
+  MK_TRY(mk::launch_w4_gemm(a, static_cast<hipStream_t>(stream)));
+}
+
 int mk_pack_weight(const void* in, int ld_in, void* out, int K, int N, int elem_bytes, int map, int ic, int inter,
                    void* stream) {
   mk::PackArgs p{};

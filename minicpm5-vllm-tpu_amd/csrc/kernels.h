@@ -125,6 +125,23 @@ struct LogprobArgs {
 size_t logprob_scratch_bytes(int T, int V, int n_ids, int top);
 int launch_logprobs(const LogprobArgs& a, void* ws, hipStream_t st);
 
+// ------------------------------------------------------------------------------ 4-bit weights
+// W (N, K) in 4 bits with a bf16 scale per row and `group` (32, 64, 128) values of K, in blocks of 16 rows x 128 values
+// (w4.hip): codes 1 KB a block, scales 16 * 128 / group a block.
+struct W4GemmArgs {
+  const uint16_t* x; size_t ldx;   // (M, K) bf16
+  const uint8_t* codes;
+  const uint16_t* scales;
+  void* out; size_t ldo;           // (M, N) f32 or bf16
+  int out_f32;
+  int M, N, K, group;
+};
+int launch_w4_gemm(const W4GemmArgs& a, hipStream_t st);
+int launch_w4_quantize(const uint16_t* w, size_t ldw, int N, int K, int group, uint8_t* codes, uint16_t* scales,
+                       hipStream_t st);
+int launch_w4_dequantize(const uint8_t* codes, const uint16_t* scales, int N, int K, int group, void* out, bool f32,
+                         size_t ldo, hipStream_t st);
+
 // ------------------------------------------------------------------------------ norm / quant
 // Activation quantisation of rows x (T, H), one kernel for the reference's four activation modes
 // (qmax = 127 for int8, 448 for fp8 e4m3; rstd = rsqrt(mean(x^2) + eps) with norm, else 1):

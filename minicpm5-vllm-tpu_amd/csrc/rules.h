@@ -154,4 +154,13 @@ inline LogprobPlan logprob_plan(int T, int V) {
   return {most < room ? most : room, 16};
 }
 
+// How the 4-bit product divides nrb blocks of 16 weight rows: r blocks a wave, K dealt to kw of a workgroup's 8 waves.
+struct W4Plan { int r, kw; };
+inline W4Plan w4_plan(long nrb, int nkb) {
+  if (nrb >= 16 * 256) return {2, 1};
+  int kw = 1;
+  while (kw < 8 && nrb * kw < 8 * 256 && kw * 2 <= nkb) kw *= 2;
+  return {1, kw};
+}
+
 }  // namespace mk

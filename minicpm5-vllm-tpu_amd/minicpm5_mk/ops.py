@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
@@ -261,6 +262,80 @@ def logprobs(logits: torch.Tensor, ids: torch.Tensor | None = None, top: int = 0
     return LogProbs(lp, rk, tl, ti, ent, lse)
 
 
+@dataclass(frozen=True)
+class W4Weight:
+    """A weight (n, k) in 4 bits with a bf16 scale per row and `group` values of k, in libmk's block layout
+    (include/mk.h, mk_w4_quantize).  Made by quantize_w4."""
+    codes: torch.Tensor    # uint8
+    scales: torch.Tensor   # bf16
+    n: int
+    k: int
+    group: int
+
+
+def _w4_sizes(n: int, k: int, group: int):
+    codes, scales = ctypes.c_size_t(), ctypes.c_size_t()
+    check(load().mk_w4_bytes(n, k, group, ctypes.byref(codes), ctypes.byref(scales)), "mk_w4_bytes")
+    return codes.value, scales.value
+
+
+def _need_w4(w):
+    if not isinstance(w, W4Weight):
+        raise MkError("expected a W4Weight (quantize_w4)")
+
+
+def quantize_w4(weight: torch.Tensor, group: int = 128) -> W4Weight:
+    """weight (N, K) bf16 -> 4-bit codes in [-7, 7] under a bf16 scale amax / 7 per row and `group` (32, 64 or 128)
+    values of K.  Any N and K; rows may be strided.  A group with a NaN or an infinity gets a NaN scale."""
+    lib = load()
+    _need_rows(weight, "weight", (BF16,))
+    n, k = weight.shape
+    nc, ns = _w4_sizes(n, k, int(group))
+    with _on(weight):
+        codes = torch.empty(nc, dtype=torch.uint8, device=weight.device)
+        scales = torch.empty(ns // 2, dtype=BF16, device=weight.device)
+        check(lib.mk_w4_quantize(_adr(weight), weight.stride(0), n, k, group, _adr(codes), _adr(scales), _raw_stream()),
+              "mk_w4_quantize")
+    return W4Weight(codes, scales, n, k, int(group))
+
+
+def dequantize_w4(w: W4Weight, dtype: torch.dtype = BF16) -> torch.Tensor:
+    """The values a W4Weight stands for: (N, K) f32 (exact) or bf16 (rounded once)."""
+    lib = load()
+    _need_w4(w)
+    if dtype not in (BF16, torch.float32):
+        raise MkError(f"dequantize_w4: dtype {dtype}, expected bf16 or f32")
+    with _on(w.codes):
+        out = torch.empty((w.n, w.k), dtype=dtype, device=w.codes.device)
+        check(lib.mk_w4_dequantize(_adr(w.codes), _adr(w.scales), w.n, w.k, w.group, _adr(out), int(dtype != BF16), w.k,
+                                   _raw_stream()), "mk_w4_dequantize")
+    return out
+
+
+def gemm_w4(x: torch.Tensor, w: W4Weight, dtype: torch.dtype = BF16, out: torch.Tensor | None = None) -> torch.Tensor:
+    """x (M, K) bf16 @ w (N, K)^T with 4-bit weights, f32 accumulation -> (M, N) bf16 or f32 (include/mk.h, mk_gemm_w4).
+
+    For few rows: the weights are read once per 64 rows of x.  x and `out` may have strided rows."""
+    lib = load()
+    _need_w4(w)
+    _need_rows(x, "x", (BF16,), w.k)
+    M = x.shape[0]
+    if out is None:
+        if dtype not in (BF16, torch.float32):
+            raise MkError(f"gemm_w4: dtype {dtype}, expected bf16 or f32")
+    else:
+        _need_rows(out, "out", (BF16, torch.float32), w.n)
+        if out.shape[0] != M:
+            raise MkError(f"out: {out.shape[0]} rows, expected {M}")
+    _same_device(x, w=w.codes, out=out)
+    with _on(x):
+        if out is None:
+            out = torch.empty((M, w.n), dtype=dtype, device=x.device)
+        check(lib.mk_gemm_w4(_adr(x), x.stride(0), _adr(w.codes), _adr(w.scales), M, w.n, w.k, w.group, _adr(out),
+                             int(out.dtype != BF16), out.stride(0), _raw_stream()), "mk_gemm_w4")
+    return out
+
+
 def pack_weight(w: torch.Tensor, map_gu: bool = False, ic: int = 0, inter: int = 0) -> torch.Tensor:
     """(K, N) -> (N, K) repack (the layout mk_model_create builds); map_gu reorders gate/up columns."""
     lib = load()
@@ -273,4 +348,4 @@ def pack_weight(w: torch.Tensor, map_gu: bool = False, ic: int = 0, inter: int =
 
 
 __all__ = ["attn_prefill", "attn_scratch_bytes", "row_quant", "act_quant", "gemm", "lm_head", "logprobs", "LogProbs",
-           "pack_weight", "MkError", "_lib"]
+           "W4Weight", "quantize_w4", "dequantize_w4", "gemm_w4", "pack_weight", "MkError", "_lib"]

@@ -56,3 +56,65 @@ def test_logprobs_cpu_tensor():
         ops.logprobs(torch.zeros(2, 8))
     with pytest.raises(_lib.MkError, match="torch.Tensor"):
         ops.logprobs([[0.0]])
+
+
+def _w4(name, **kw):
+    lib = _lib.load()
+    d = dict(x=BOGUS, ldx=256, w=BOGUS, ldw=256, codes=BOGUS, scales=BOGUS, M=2, N=100, K=256, group=64, out=BOGUS, f32=0,
+             ldo=256)
+    d.update(kw)
+    if name == "quantize":
+        return lib.mk_w4_quantize(d["w"], d["ldw"], d["N"], d["K"], d["group"], d["codes"], d["scales"], None)
+    if name == "dequantize":
+        return lib.mk_w4_dequantize(d["codes"], d["scales"], d["N"], d["K"], d["group"], d["out"], d["f32"], d["ldo"], None)
+    return lib.mk_gemm_w4(d["x"], d["ldx"], d["codes"], d["scales"], d["M"], d["N"], d["K"], d["group"], d["out"], d["f32"],
+                          d["ldo"], None)
+
+
+@pytest.mark.parametrize("name,kw,code,msg", [
+    *[(n, dict(group=g), -1, "group") for n in ("quantize", "dequantize", "gemm") for g in (0, 16, 96, 256)],
+    *[(n, kw, -1, "empty") for n in ("quantize", "dequantize", "gemm") for kw in (dict(N=0), dict(K=0))],
+    *[(n, dict(codes=None), -1, "null") for n in ("quantize", "dequantize", "gemm")],
+    *[(n, dict(scales=BOGUS + 16), -1, "32-byte") for n in ("quantize", "dequantize", "gemm")],
+    *[(n, dict(N=1 << 30, K=1 << 30, ldw=1 << 30, ldx=1 << 30, ldo=1 << 30), -1, "large")
+      for n in ("quantize", "dequantize", "gemm")],
+    ("quantize", dict(w=None), -1, "null"),
+    ("quantize", dict(ldw=255), -1, "stride"),
+    ("dequantize", dict(out=BOGUS + 2, f32=1), -1, "misaligned"),
+    ("dequantize", dict(ldo=255), -1, "stride"),
+    ("gemm", dict(M=-1), -1, "negative"),
+    ("gemm", dict(x=None), -1, "null"),
+    ("gemm", dict(x=BOGUS + 1), -1, "misaligned"),
+    ("gemm", dict(ldx=255), -1, "stride"),
+    ("gemm", dict(ldo=99), -1, "stride"),
+    ("gemm", dict(M=0), 0, ""),
+])
+def test_w4_refusals(name, kw, code, msg):
+    assert _w4(name, **kw) == code
+    if code:
+        assert msg in _err()
+
+
+def test_w4_bytes():
+    c, s = ctypes.c_size_t(), ctypes.c_size_t()
+    f = _lib.load().mk_w4_bytes
+    assert f(33, 130, 32, ctypes.byref(c), ctypes.byref(s)) == 0
+    assert (c.value, s.value) == (3 * 2 * 1024, 3 * 2 * 16 * 4 * 2)
+    assert f(130560, 1536, 128, ctypes.byref(c), ctypes.byref(s)) == 0
+    assert (c.value, s.value) == (130560 * 1536 // 2, 130560 * 12 * 2)
+    assert f(1, 1, 32, None, None) == -1
+
+
+def test_w4_cpu_tensors():
+    with pytest.raises(_lib.MkError, match="GPU tensor"):
+        ops.quantize_w4(torch.zeros(4, 64, dtype=torch.bfloat16))
+    with pytest.raises(_lib.MkError, match="W4Weight"):
+        ops.gemm_w4(torch.zeros(1, 64, dtype=torch.bfloat16), torch.zeros(4, 64))
+    with pytest.raises(_lib.MkError, match="W4Weight"):
+        ops.dequantize_w4(None)
+    z = torch.zeros(1024, dtype=torch.uint8)
+    w = ops.W4Weight(z, z.bfloat16(), 4, 64, 64)
+    with pytest.raises(_lib.MkError, match="dtype"):
+        ops.dequantize_w4(w, dtype=torch.float16)
+    with pytest.raises(_lib.MkError, match="GPU tensor"):
+        ops.gemm_w4(torch.zeros(1, 64, dtype=torch.bfloat16), w)
