@@ -273,6 +273,15 @@ int mk_logprobs(const void* logits, int type, size_t ld, int T, int V, const voi
                 float* token_lp, int32_t* ranks, float* top_lp, int32_t* top_ids, float* entropy, float* lse,
                 void* scratch, size_t scratch_bytes, void* stream);
 
+/* mk_logprobs of the logits hidden (T, H) weight (V, H)^T (bf16, contiguous, f32 accumulation): token_lp, entropy and
+ * lse as there, without ranks and alternatives.  Of more than 64 rows no logit is stored, only statistics of 256 tokens
+ * of the vocabulary at a time.  H a multiple of 32; hidden, weight and scratch 16-byte aligned; scratch:
+ * mk_lm_head_logprobs_scratch_bytes bytes (101 MB at most for V = 130560), not shared by calls that overlap.  A row's
+ * results may differ in the last bits with the number of rows, as they are made in another order. */
+size_t mk_lm_head_logprobs_scratch_bytes(int T, int V, int n_ids);
+int mk_lm_head_logprobs(const void* hidden, const void* weight, int T, int H, int V, const void* ids, int ids64, int n_ids,
+                        float* token_lp, float* entropy, float* lse, void* scratch, size_t scratch_bytes, void* stream);
+
 /* 4-bit weights with group scales (no counterpart in the reference).  W (N, K) bf16, row stride ldw elements; along K
  * each row is cut into groups of `group` (32, 64 or 128) values, the last one shorter.  Of a group:
  *   s = bf16(amax / 7), 0 where amax / 7 < 2^-126, NaN where a value is not finite;

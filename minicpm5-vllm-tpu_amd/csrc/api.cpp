@@ -361,6 +361,30 @@ int mk_logprobs(const void* logits, int type, size_t ld, int T, int V, const voi
   MK_TRY(mk::launch_logprobs(a, scratch, static_cast<hipStream_t>(stream)));
 }
 
+size_t mk_lm_head_logprobs_scratch_bytes(int T, int V, int n_ids) {
+  if (T < 1 || V < 1 || n_ids < 0) return 0;
+  return mk::head_logprob_scratch_bytes(T, V, n_ids);
+}
+
+int mk_lm_head_logprobs(const void* hidden, const void* weight, int T, int H, int V, const void* ids, int ids64, int n_ids,
+                        float* token_lp, float* entropy, float* lse, void* scratch, size_t scratch_bytes, void* stream) {
+  MK_REQUIRE(T >= 0 && V >= 1 && V <= (1 << 30), "lm_head_logprobs: T must be >= 0 and V in 1 .. 2^30");
+  MK_REQUIRE(H >= 32 && H % 32 == 0 && H <= (1 << 20), "lm_head_logprobs: H must be a multiple of 32");
+  MK_REQUIRE(n_ids >= 0 && n_ids <= mk::LP_MAX_IDS, "lm_head_logprobs: at most 64 given tokens a row");
+  if (T == 0) return MK_OK;
+  MK_REQUIRE(hidden && weight && entropy && lse, "lm_head_logprobs: null pointer");
+  MK_REQUIRE(n_ids == 0 || (ids && token_lp), "lm_head_logprobs: null pointer of the given tokens");
+  MK_REQUIRE(aligned16(hidden) && aligned16(weight), "lm_head_logprobs: hidden and weight must be 16-byte aligned");
+  if (!scratch || scratch_bytes < mk::head_logprob_scratch_bytes(T, V, n_ids)) {
+    mk::set_error("lm_head_logprobs: scratch too small");
+    return MK_ENOMEM;
+  }
+  MK_REQUIRE(aligned16(scratch), "lm_head_logprobs: scratch must be 16-byte aligned");
+  const mk::HeadLogprobArgs a{static_cast<const uint16_t*>(hidden), static_cast<const uint16_t*>(weight), ids, ids64 != 0,
+                              n_ids, T, H, V, token_lp, entropy, lse};
+  MK_TRY(mk::launch_head_logprobs(a, scratch, static_cast<hipStream_t>(stream)));
+}
+
 namespace {
 bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 

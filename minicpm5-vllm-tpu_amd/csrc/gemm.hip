@@ -1023,6 +1023,73 @@ __global__ __launch_bounds__(block_threads(WGM, WGN, LOOP), OCC) void gemm_kerne
   if constexpr (RES) load_res(0, rv[0]);
   if (!EARLY_SCALES && dq) load_scales();
   lds_barrier();   // every wave is done reading the LDS ring
+  if constexpr (EPI == Epi::LSE) {
+    // Statistics of the tile's columns (tokens) over its rows (vocabulary).  A lane holds 16 MT rows of one column of
+    // each 32-column tile, so the sums run in registers; the other half of the rows is lane ^ 32's, other waves' come
+    // through LDS.  In log2: one fma makes the exponent, and the reference need not be the exact maximum.  Rows past M
+    // (copies of the last one) are taken out.
+    constexpr float LOG2E = 1.4426950408889634f, OUT = -1.5e38f;   // times LOG2E still finite
+    float* red = reinterpret_cast<float*>(smem);   // [WGM][3][BN]
+    const int mw = m0 + wm * C::WM;
+    if (mw + C::WM > g.M) {
+#pragma unroll
+      for (int mt = 0; mt < C::MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (mw + 32 * mt + 8 * (r >> 2) + 4 * half + (r & 3) >= g.M) {
+#pragma unroll
+            for (int nt = 0; nt < C::NTL; ++nt) acc[mt][nt][r] = OUT;
+          }
+    }
+#pragma unroll
+    for (int nt = 0; nt < C::NTL; ++nt) {
+      float mx = acc[0][nt][0];
+#pragma unroll
+      for (int mt = 0; mt < C::MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, acc[mt][nt][r]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float ref = fmaxf(mx, -1e38f) * LOG2E;
+      float s[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int mt = 0; mt < C::MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float t = fmaf(acc[mt][nt][r], LOG2E, -ref), p = fast_exp2(t);
+          s[r & 3] += p;
+          u[r & 3] = fmaf(p, t, u[r & 3]);
+        }
+      float ss = (s[0] + s[1]) + (s[2] + s[3]), uu = (u[0] + u[1]) + (u[2] + u[3]);
+      ss += __shfl_xor(ss, 32);
+      uu += __shfl_xor(uu, 32);
+      if (half == 0) {
+        float* o = red + wm * 3 * BN + wn * C::WN + 32 * nt + col;
+        o[0] = ref;
+        o[BN] = ss;
+        o[2 * BN] = uu;
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    lds_barrier();
+    for (int n = tid; n < BN && n0 + n < g.N; n += C::NTH) {
+      float ref = red[n];
+#pragma unroll
+      for (int k = 1; k < C::WGM; ++k) ref = fmaxf(ref, red[k * 3 * BN + n]);
+      float ss = 0.f, uu = 0.f;
+#pragma unroll
+      for (int k = 0; k < C::WGM; ++k) {
+        const float* o = red + k * 3 * BN + n;
+        const float d = fmaxf(o[0] - ref, -1e4f), f = fast_exp2(d);
+        ss = fmaf(f, o[BN], ss);
+        uu = fmaf(f, fmaf(d, o[BN], o[2 * BN]), uu);
+      }
+      float* o = static_cast<float*>(g.out) + (size_t)(m0 / BM) * 3 * g.ldo + n0 + n;
+      o[0] = ref;
+      o[g.ldo] = ss;
+      o[2 * (size_t)g.ldo] = uu;
+    }
+    return;
+  } else {
   constexpr int EROW = C::EROW;
   char* er = smem + w * 32 * EROW;
   using V4 = typename T::Vec4;
@@ -1244,6 +1311,7 @@ __global__ __launch_bounds__(block_threads(WGM, WGN, LOOP), OCC) void gemm_kerne
     }
     __builtin_amdgcn_wave_barrier();
     }
+  }
   }
 }
 
@@ -1606,6 +1674,7 @@ void launch_skinny_t(const GemmArgs& g, hipStream_t st) {
 // fp8 / fp8d linears (and F32 for tests); the bf16 GEMMs never dequantise a residual in bf16.
 template <GemmIn IN>
 constexpr bool epi_built(Epi e) {
+  if (e == Epi::LSE) return false;   // launch_gemm_lse
   if constexpr (IN == GemmIn::F8)
     return e == Epi::F32 || e == Epi::DQ_BF16 || e == Epi::DQ2_BF16 || e == Epi::DQ_RES_BF16ADD ||
            e == Epi::DQ2_RES_BF16ADD || e == Epi::SILU_BF16;
@@ -1656,6 +1725,7 @@ int dispatch(const GemmArgs& g, hipStream_t st, bool skinny) {
     MK_CASE(SILU_BF16)
     MK_CASE(DQ_SILU)
     MK_CASE(DQ_SILU_F32A)
+    case Epi::LSE: break;
   }
 #undef MK_CASE
   set_error("gemm: unknown epilogue");
@@ -1722,6 +1792,24 @@ int launch_gemm(const GemmArgs& g, hipStream_t st) {
     case GemmIn::F8: return dispatch<GemmIn::F8>(g, st, false);
     default: return dispatch<GemmIn::BF16>(g, st, false);
   }
+}
+
+int launch_gemm_lse(const GemmArgs& g0, hipStream_t st) {
+  GemmArgs g = g0;
+  g.in = GemmIn::BF16;
+  g.epi = Epi::LSE;
+  int rc = gemm_validate(g);
+  if (rc) return rc;
+  MK_REQUIRE(g.K % 32 == 0 && g.ldo >= g.N, "gemm_lse: K must be a multiple of 32 and ldo at least N");
+  static_assert(CfgM::BM == LSE_ROWS && CfgN::BM == LSE_ROWS && CfgX::BM == LSE_ROWS && CfgW4::BM == LSE_ROWS, "one statistic per 256 rows, whatever the tile");
+  switch (lse_tile(g.N)) {
+    case 2: launch_c<CfgM, GemmIn::BF16, Epi::LSE>(g, st); break;
+    case 5: launch_c<CfgN, GemmIn::BF16, Epi::LSE>(g, st); break;
+    case 8: launch_c<CfgW4, GemmIn::BF16, Epi::LSE>(g, st); break;
+    default: launch_c<CfgX, GemmIn::BF16, Epi::LSE>(g, st); break;
+  }
+  MK_HIP_CHECK(hipGetLastError());
+  return MK_OK;
 }
 
 int launch_gemm_skinny(const GemmArgs& g, hipStream_t st) {

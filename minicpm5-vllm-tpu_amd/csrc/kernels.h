@@ -63,6 +63,7 @@ enum class Epi {
   SILU_BF16,      // g/u interleaved: g, u = bf16(acc [* (rs[m] * cs[n])]); h = bf16(bf16(silu(g)) * u)
   DQ2_BF16,       // out = bf16(acc * (rs[m] * cs[n]))                     (linear_rmsnorm int8d)
   DQ2_RES_BF16ADD,// res = bf16(res + bf16(acc * (rs[m] * cs[n])))          (fp8d O / down projection)
+  LSE,            // f32 statistics of each column n over the tile's rows, bf16 operands (launch_gemm_lse)
 };
 struct GemmArgs {
   GemmIn in;
@@ -103,6 +104,11 @@ int launch_gemm(const GemmArgs& g, hipStream_t st);
 int launch_gemm_skinny(const GemmArgs& g, hipStream_t st);
 // Logits (F32 epilogue, bf16 operands) of any number of rows, the weights read once per 64 of them.
 int launch_lm_head(const GemmArgs& g, hipStream_t st);
+// Softmax statistics of C(M, N) = A B^T over its rows (M: vocabulary, N: tokens; bf16), C itself not stored.  Of every
+// LSE_ROWS rows t and column n: out[(3 t + 0) ldo + n] = a reference exponent r, [3 t + 1] sum 2^(C log2 e - r),
+// [3 t + 2] sum 2^(C log2 e - r) (C log2 e - r).
+constexpr int LSE_ROWS = 256;
+int launch_gemm_lse(const GemmArgs& g, hipStream_t st);
 
 // ------------------------------------------------------------------------------ log probabilities
 // Rows x (T, V) at row stride ldx (elements): log p of n_ids given tokens a row with their ranks, entropy, log of the
@@ -116,7 +122,7 @@ struct LogprobArgs {
   int ids64, n_ids;
   int T, V, top;
   float* token_lp;       // (T, n_ids)
-  int* ranks;            // (T, n_ids)
+  int* ranks;            // (T, n_ids); null: not counted
   float* top_lp;         // (T, top)
   int* top_ids;          // (T, top)
   float* entropy;        // (T)
@@ -124,6 +130,20 @@ struct LogprobArgs {
 };
 size_t logprob_scratch_bytes(int T, int V, int n_ids, int top);
 int launch_logprobs(const LogprobArgs& a, void* ws, hipStream_t st);
+// The same of the logits hidden (T, H) weight (V, H)^T, bf16, without ranks and alternatives; the logits of many rows
+// are never stored.
+struct HeadLogprobArgs {
+  const uint16_t* hidden;
+  const uint16_t* weight;
+  const void* ids;
+  int ids64, n_ids;
+  int T, H, V;
+  float* token_lp;
+  float* entropy;
+  float* lse;
+};
+size_t head_logprob_scratch_bytes(int T, int V, int n_ids);
+int launch_head_logprobs(const HeadLogprobArgs& a, void* ws, hipStream_t st);
 
 // ------------------------------------------------------------------------------ 4-bit weights
 // W (N, K) in 4 bits with a bf16 scale per row and `group` (32, 64, 128) values of K, in blocks of 16 rows x 128 values

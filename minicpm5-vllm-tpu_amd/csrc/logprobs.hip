@@ -259,7 +259,7 @@ struct RowOut {
   __device__ void token(const LogprobArgs& a, int row, int j, bool in, float v, int above) const {
     const size_t o = (size_t)row * a.n_ids + j;
     a.token_lp[o] = nan || in ? lp(v) : neg_inf();
-    a.ranks[o] = nan || !in ? -1 : 1 + above;
+    if (a.ranks) a.ranks[o] = nan || !in ? -1 : 1 + above;
   }
   __device__ void top(const LogprobArgs& a, int row, int place, u64 e) const {
     const size_t o = (size_t)row * a.top + place;
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 6) void logprob_rows_
     st.s += s;
     st.u += u;
 
-    for (int j = 0; j < a.n_ids; ++j) {
+    for (int j = 0; a.ranks && j < a.n_ids; ++j) {
       const float jv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(iv), j));
       const int ji = __builtin_amdgcn_readlane(id, j);
       int n = 0;
@@ -519,6 +519,72 @@ int launch_t(const LogprobArgs& a, void* ws, hipStream_t st) {
   return MK_OK;
 }
 
+// ------------------------------------------------------------------------------------------------ from hidden states
+// The rows' log probabilities from the statistics the LM head product leaves (launch_gemm_lse): a workgroup merges 16 rows'
+// `tiles` entries, 16 threads a row, and makes the given tokens' logits as dot products of f32 sums, a wave each.
+constexpr int HF_ROWS = 16, HF_PARTS = 16;
+
+__global__ __launch_bounds__(256) void head_finish_kernel(HeadLogprobArgs a, int tiles, const float* part) {
+  __shared__ float sh[3][HF_PARTS][HF_ROWS];
+  __shared__ double lse[HF_ROWS];
+  const int r = threadIdx.x % HF_ROWS, q = threadIdx.x / HF_ROWS, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int row0 = blockIdx.x * HF_ROWS, row = row0 + r;
+  // log2 units: m a reference exponent, as the tiles' are
+  float m = NEG_MAX, s = 0.f, u = 0.f;
+  auto merge = [&](float m2, float s2, float u2) {
+    const float mn = fmaxf(m, m2), d1 = fmaxf(m - mn, -1e4f), d2 = fmaxf(m2 - mn, -1e4f);
+    const float f1 = fast_exp2(d1), f2 = fast_exp2(d2);
+    u = f1 * fmaf(d1, s, u) + f2 * fmaf(d2, s2, u2);
+    s = f1 * s + f2 * s2;
+    m = mn;
+  };
+  const float* p = part + min(row, a.T - 1);
+#pragma unroll 4
+  for (int t = q; t < tiles; t += HF_PARTS) {
+    const float* e = p + (size_t)t * 3 * a.T;
+    merge(e[0], e[a.T], e[2 * (size_t)a.T]);
+  }
+  sh[0][q][r] = m;
+  sh[1][q][r] = s;
+  sh[2][q][r] = u;
+  __syncthreads();
+  if (q == 0) {
+#pragma unroll
+    for (int o = 1; o < HF_PARTS; ++o) merge(sh[0][o][r], sh[1][o][r], sh[2][o][r]);
+    const double ln2 = 0.6931471805599453, l2 = (double)log2f(s);
+    lse[r] = ((double)m + l2) * ln2;
+    if (row < a.T) {
+      a.lse[row] = (float)lse[r];
+      a.entropy[row] = (float)((l2 - (double)(u / s)) * ln2);
+    }
+  }
+  __syncthreads();
+  for (int i = w; i < HF_ROWS * a.n_ids; i += 4) {
+    const int rr = row0 + i / a.n_ids;
+    if (rr >= a.T) break;
+    const size_t o = (size_t)rr * a.n_ids + i % a.n_ids;
+    const long long id = a.ids64 ? static_cast<const long long*>(a.ids)[o] : static_cast<const int*>(a.ids)[o];
+    const bool in = id >= 0 && id < a.V;
+    const uint16_t *h = a.hidden + (size_t)rr * a.H, *wt = a.weight + (size_t)(in ? id : 0) * a.H;
+    float d = 0.f;
+    for (int k = lane * 8; k < a.H; k += 512) {
+      const u32x4 hv = *reinterpret_cast<const u32x4*>(h + k), wv = *reinterpret_cast<const u32x4*>(wt + k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        d = fmaf(bf_lo(hv[e]), bf_lo(wv[e]), d);
+        d = fmaf(bf_hi(hv[e]), bf_hi(wv[e]), d);
+      }
+    }
+    d = wave_sum(d);
+    const double l = lse[rr - row0];
+    // a NaN row is NaN for every id; rounding may put a certain token a step above 0
+    if (lane == 0) a.token_lp[o] = !(l == l) ? __builtin_nanf("") : in ? fminf((float)((double)d - l), 0.f) : neg_inf();
+  }
+}
+
+// Rows of a pass over the vocabulary that keeps statistics only: 16384, 100 MB of them at V = 130560.
+constexpr int HEAD_PASS = 16384;
+
 }  // namespace
 
 size_t logprob_scratch_bytes(int T, int V, int n_ids, int top) {
@@ -535,6 +601,62 @@ int launch_logprobs(const LogprobArgs& a, void* ws, hipStream_t st) {
   }
   set_error("logprobs: unknown logits type");
   return MK_EINVAL;
+}
+
+size_t head_logprob_scratch_bytes(int T, int V, int n_ids) {
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  if (head_logprobs_stored(T)) return up((size_t)T * V * sizeof(float)) + logprob_scratch_bytes(T, V, n_ids, 0);
+  return (size_t)((V + LSE_ROWS - 1) / LSE_ROWS) * 3 * std::min(T, HEAD_PASS) * sizeof(float);
+}
+
+int launch_head_logprobs(const HeadLogprobArgs& a, void* ws, hipStream_t st) {
+  // the products take operands under 4 GiB: the vocabulary in slices of whole tiles
+  const int slice = (int)std::min<size_t>(a.V, ((((size_t)1 << 32) - 1) / ((size_t)a.H * 2)) / LSE_ROWS * LSE_ROWS);
+  MK_REQUIRE(slice >= 1, "lm_head_logprobs: H too large");
+  GemmArgs g{};
+  g.in = GemmIn::BF16;
+  g.K = g.lda = g.ldb = a.H;
+  if (head_logprobs_stored(a.T)) {
+    float* logits = static_cast<float*>(ws);
+    g.epi = Epi::F32;
+    g.A = a.hidden;
+    g.M = a.T;
+    g.ldo = a.V;
+    for (int v0 = 0; v0 < a.V; v0 += slice) {
+      g.B = a.weight + (size_t)v0 * a.H;
+      g.N = std::min(slice, a.V - v0);
+      g.out = logits + v0;
+      const int rc = launch_lm_head(g, st);
+      if (rc) return rc;
+    }
+    LogprobArgs l{logits, (size_t)a.V, 0, a.ids, a.ids64, a.n_ids, a.T, a.V, 0, a.token_lp, nullptr, nullptr, nullptr,
+                  a.entropy, a.lse};
+    return launch_logprobs(l, static_cast<char*>(ws) + ((size_t)a.T * a.V * sizeof(float) + 255) / 256 * 256, st);
+  }
+  const int tiles = (a.V + LSE_ROWS - 1) / LSE_ROWS;
+  for (int t0 = 0; t0 < a.T; t0 += HEAD_PASS) {
+    HeadLogprobArgs h = a;
+    h.T = std::min(HEAD_PASS, a.T - t0);
+    h.hidden = a.hidden + (size_t)t0 * a.H;
+    const size_t at = (size_t)t0 * a.n_ids;
+    h.ids = static_cast<const char*>(a.ids) + at * (a.ids64 ? 8 : 4);
+    h.token_lp = a.token_lp + at;
+    h.entropy = a.entropy + t0;
+    h.lse = a.lse + t0;
+    g.B = h.hidden;
+    g.N = g.ldo = h.T;
+    for (int v0 = 0; v0 < a.V; v0 += slice) {
+      g.A = a.weight + (size_t)v0 * a.H;
+      g.M = std::min(slice, a.V - v0);
+      g.out = static_cast<float*>(ws) + (size_t)(v0 / LSE_ROWS) * 3 * h.T;
+      const int rc = launch_gemm_lse(g, st);
+      if (rc) return rc;
+    }
+    hipLaunchKernelGGL(head_finish_kernel, dim3((h.T + HF_ROWS - 1) / HF_ROWS), dim3(256), 0, st, h, tiles,
+                       static_cast<const float*>(ws));
+    MK_HIP_CHECK(hipGetLastError());
+  }
+  return MK_OK;
 }
 
 }  // namespace mk

@@ -163,4 +163,30 @@ inline W4Plan w4_plan(long nrb, int nkb) {
   return {1, kw};
 }
 
+// GEMM tile (256 of the vocabulary x 128, 192, 256 or 320 tokens) of the LM head product that keeps statistics only:
+// the least tokens of whole tiles by the tiles' rate.  Measured at V = 130560, H = 1536, us on 256x128, 256x192, 256x256,
+// 256x320 tiles: 128 tokens 105, 116, 125, 136; 192 143, 115, 119, 130; 256 145, 174, 121, 133; 320 221, 179, 183, 137;
+// 384 227, 183, 188, 224; 512 248, 250, 203, 230; 640 293, 309, 288, 246; 768 360, 317, 295, 341; 8192 3160, 2971, 2603,
+// 2754.
+inline int lse_tile(int T) {
+  struct Opt { int id, bn; double eff; };
+  const Opt opts[4] = {{4, 256, 1.33}, {8, 320, 1.26}, {5, 192, 1.13}, {2, 128, 1.095}};
+  int best = 4;
+  double least = 1e300;
+  for (const Opt& o : opts) {
+    const double t = (double)((T + o.bn - 1) / o.bn) * o.bn / o.eff;
+    if (t < least * 0.999) {
+      least = t;
+      best = o.id;
+    }
+  }
+  return best;
+}
+
+// Whether the log probabilities of T hidden rows go through stored logits (the LM head's kernels for up to 64 rows, then
+// a pass over them) and not through the tiled product that keeps statistics only.  us, stored then tiled: V = 130560,
+// H = 1536, 16 rows 85, 96, 40 rows 93, 94, 64 rows 100, 95; H = 2048, 64 rows 126, 139; V = 32768, 64 rows 27, 38,
+// 100 rows (two passes of the head) 46, 38; V = 8000, 64 rows 22, 27, 100 rows 37, 27.
+inline bool head_logprobs_stored(int T) { return T <= 64; }
+
 }  // namespace mk

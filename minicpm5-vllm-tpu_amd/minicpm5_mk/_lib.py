@@ -68,6 +68,8 @@ SIGNATURES = {
     "mk_lm_head": (_I, [_P, _P, _I, _I, _I, _P, _P]),
     "mk_logprobs_scratch_bytes": (_SZ, [_I, _I, _I, _I]),
     "mk_logprobs": (_I, [_P, _I, _SZ, _I, _I, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "mk_lm_head_logprobs_scratch_bytes": (_SZ, [_I, _I, _I]),
+    "mk_lm_head_logprobs": (_I, [_P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _P, _P, _SZ, _P]),
     "mk_w4_bytes": (_I, [_I, _I, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)]),
     "mk_w4_quantize": (_I, [_P, _SZ, _I, _I, _I, _P, _P, _P]),
     "mk_w4_dequantize": (_I, [_P, _P, _I, _I, _I, _P, _I, _SZ, _P]),

@@ -262,6 +262,34 @@ def logprobs(logits: torch.Tensor, ids: torch.Tensor | None = None, top: int = 0
     return LogProbs(lp, rk, tl, ti, ent, lse)
 
 
+def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, ids: torch.Tensor | None = None) -> LogProbs:
+    """logprobs(lm_head(hidden, weight), ids) without ranks and alternatives, and for more than 64 rows without the
+    logits: hidden (T, H) bf16, weight (V, H) bf16, H a multiple of 32 (include/mk.h, mk_lm_head_logprobs).
+
+    For the tokens of whole prompts: a (8192, 130560) f32 matrix of logits is 4.3 GB.  No gradient."""
+    lib = load()
+    _need(hidden, "hidden", BF16)
+    if hidden.dim() != 2 or not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise MkError("lm_head_logprobs: expected hidden (T, H) and weight (V, H)")
+    T, H = hidden.shape
+    V = weight.shape[0]
+    _need(weight, "weight", BF16, (V, H))
+    if V < 1:
+        raise MkError("weight: empty vocabulary")
+    n = 0 if ids is None else _need_ids(ids, T)
+    _same_device(hidden, weight=weight, ids=ids)
+    dev = hidden.device
+    with _on(hidden):
+        lp = None if ids is None else torch.empty(ids.shape, dtype=torch.float32, device=dev)
+        ent, lse = torch.empty((2, T), dtype=torch.float32, device=dev).unbind()
+        nbytes = int(lib.mk_lm_head_logprobs_scratch_bytes(T, V, n))
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        check(lib.mk_lm_head_logprobs(_adr(hidden), _adr(weight), T, H, V, _adr(ids),
+                                      int(n > 0 and ids.dtype == torch.int64), n, _adr(lp), _adr(ent), _adr(lse),
+                                      _adr(scratch), nbytes, _raw_stream()), "mk_lm_head_logprobs")
+    return LogProbs(lp, None, None, None, ent, lse)
+
+
 @dataclass(frozen=True)
 class W4Weight:
     """A weight (n, k) in 4 bits with a bf16 scale per row and `group` values of k, in libmk's block layout
@@ -347,5 +375,5 @@ def pack_weight(w: torch.Tensor, map_gu: bool = False, ic: int = 0, inter: int =
     return out
 
 
-__all__ = ["attn_prefill", "attn_scratch_bytes", "row_quant", "act_quant", "gemm", "lm_head", "logprobs", "LogProbs",
+__all__ = ["attn_prefill", "attn_scratch_bytes", "row_quant", "act_quant", "gemm", "lm_head", "logprobs", "LogProbs", "lm_head_logprobs",
            "W4Weight", "quantize_w4", "dequantize_w4", "gemm_w4", "pack_weight", "MkError", "_lib"]

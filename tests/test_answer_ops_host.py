@@ -58,6 +58,42 @@ def test_logprobs_cpu_tensor():
         ops.logprobs([[0.0]])
 
 
+def _head(**kw):
+    a = dict(hidden=BOGUS, weight=BOGUS, T=100, H=64, V=1000, ids=BOGUS, ids64=0, n_ids=1, token_lp=BOGUS, entropy=BOGUS,
+             lse=BOGUS, scratch=BOGUS, scratch_bytes=1 << 30)
+    a.update(kw)
+    return _lib.load().mk_lm_head_logprobs(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,code,msg", [
+    (dict(T=-1), -1, "T must be"),
+    (dict(V=0), -1, "V"),
+    (dict(H=0), -1, "multiple of 32"),
+    (dict(H=48), -1, "multiple of 32"),
+    (dict(n_ids=65), -1, "given tokens"),
+    (dict(hidden=None), -1, "null"),
+    (dict(token_lp=None), -1, "given tokens"),
+    (dict(hidden=BOGUS + 8), -1, "16-byte"),
+    (dict(weight=BOGUS + 2), -1, "16-byte"),
+    (dict(scratch=None), -4, "scratch"),
+    (dict(scratch_bytes=100), -4, "scratch"),
+    (dict(scratch=BOGUS + 4), -1, "16-byte"),
+    (dict(T=0), 0, ""),
+])
+def test_head_logprobs_refusals(kw, code, msg):
+    assert _head(**kw) == code
+    if code:
+        assert msg in _err()
+
+
+def test_head_logprobs_scratch():
+    f = _lib.load().mk_lm_head_logprobs_scratch_bytes
+    assert f(8192, 130560, 1) == 510 * 3 * 8192 * 4              # statistics of 256 tokens at a time
+    assert f(1 << 20, 130560, 1) == f(16384, 130560, 1)          # in passes
+    assert f(2, 1000, 1) == 8192                                 # two rows of logits, in whole 256 bytes
+    assert f(0, 1000, 1) == 0
+
+
 def _w4(name, **kw):
     lib = _lib.load()
     d = dict(x=BOGUS, ldx=256, w=BOGUS, ldw=256, codes=BOGUS, scales=BOGUS, M=2, N=100, K=256, group=64, out=BOGUS, f32=0,
