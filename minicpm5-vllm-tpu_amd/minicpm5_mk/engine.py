@@ -10,7 +10,8 @@ write (README.md:253-266, examples/minimal_vllm_inference.py:90-124):
 It serves exactly the reference plugin's fast path -- uniform fresh prefills, max_tokens == 1,
 sampling features of `sampling_fast_ok` (minicpm5_mk/__init__.py:10-32) -- and refuses anything
 else with the reference's reason codes (model.py:139-169): ragged, max_tokens,
-unsupported_sampling_feature, seq.  Weights come from an HF-named state dict (a local checkpoint)
+unsupported_sampling_feature, seq.  `MkEngine.score` answers the same batches with log probabilities of
+given tokens instead of a sample.  Weights come from an HF-named state dict (a local checkpoint)
 or the deterministic random init of `minicpm5_mk.synth`; they are prepared by `prepare_mk_weights`
 and run through libmk (`MkModel`).
 """
@@ -22,6 +23,7 @@ from dataclasses import dataclass, field
 
 import torch
 
+from . import ops
 from .config import MkConfig, preset
 from .dispatch import StepView, eligible_step, mk_seq_ok
 from .mk_weights import prepare_mk_weights
@@ -98,10 +100,34 @@ def eligible_batch(prompts, sps, max_seq: int, require_mt1: bool = True):
     return batch
 
 
+def candidate_ids(candidates, bs: int, vocab: int) -> torch.Tensor:
+    """score's candidates -> (bs, n) int64 on the host: n tokens for every prompt (a flat list) or n of each prompt's own
+    (bs lists of one length), all inside the vocabulary."""
+    t = torch.as_tensor(candidates)
+    if t.numel() and (t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool):
+        raise ValueError("candidates: expected token ids")
+    t = t.to("cpu", torch.int64)
+    if t.dim() == 1:
+        t = t.expand(bs, t.numel())
+    if t.dim() != 2 or t.shape[0] != bs:
+        raise ValueError(f"candidates: shape {tuple(t.shape)}, expected (n,) or ({bs}, n)")
+    if t.shape[1] > ops.LOGPROBS_MAX:
+        raise ValueError(f"candidates: {t.shape[1]} a prompt, at most {ops.LOGPROBS_MAX}")
+    if t.numel() and (int(t.min()) < 0 or int(t.max()) >= vocab):
+        raise ValueError(f"candidates: token ids must be in 0 .. {vocab - 1}")
+    return t.contiguous()
+
+
 class MkEngine:
+    """lm_head_quant "w4": the LM head in 4 bits (ops.quantize_w4, groups of 64 values) -- a quarter of its weight reads,
+    rounded weights; None: the bf16 head."""
+
     def __init__(self, model="1b", quant: str = "auto", state_dict: dict | None = None, weight_seed: int = 0,
-                 max_model_len: int = 8256, device: str = "cuda:0", log=print, precompile: str | None = None):
+                 max_model_len: int = 8256, device: str = "cuda:0", log=print, precompile: str | None = None,
+                 lm_head_quant: str | None = None):
         t0 = time.perf_counter()
+        if lm_head_quant not in (None, "w4"):
+            raise ValueError(f"lm_head_quant {lm_head_quant!r}: expected None or 'w4'")
         if isinstance(model, str) and os.path.isdir(model):   # local HF checkpoint directory
             from .checkpoint import load_local_checkpoint
             model, state_dict = load_local_checkpoint(model)
@@ -124,6 +150,9 @@ class MkEngine:
         self.final_norm = state_dict["model.norm.weight"].to(BF16).to(dev)
         lm = state_dict.get("lm_head.weight", state_dict["model.embed_tokens.weight"])
         self.lm_head = lm.to(BF16).to(dev)
+        self.lm_head_w4 = None
+        if lm_head_quant == "w4":
+            self.lm_head_w4, self.lm_head = ops.quantize_w4(self.lm_head, 64), None
         self.model = MkModel(self.weights, self.embed, self.cos, self.sin, self.final_norm, self.quant, cfg.n_q,
                              cfg.n_kv, cfg.head_dim, cfg.eps, lm_head=self.lm_head)
         self.counts = {"mk": 0}
@@ -136,7 +165,7 @@ class MkEngine:
         for _, s in shapes:
             if not mk_seq_ok(s, self.max_seq):
                 raise NotEligible("seq", f"precompile seq {s} not served")
-        self.model.precompile(shapes, logits=True, log=log)
+        self.model.precompile(shapes, logits=self.lm_head is not None, log=log)
 
     # ------------------------------------------------------------------ scoring
     @torch.no_grad()
@@ -150,8 +179,21 @@ class MkEngine:
         self.counts["mk"] += 1
         self.counts[key] = self.counts.get(key, 0) + 1
         self.status["shapes"].setdefault(key, {"mode": "single", "quant": self.quant})
+        if self.lm_head_w4 is not None:
+            hidden = self.model.forward(ids.reshape(-1), B, S, copy_out=False)
+            return ops.gemm_w4(hidden[:B], self.lm_head_w4, dtype=torch.float32)
         _, lg = self.model.forward(ids.reshape(-1), B, S, logits=True, copy_out=False)
         return lg
+
+    @torch.no_grad()
+    def score(self, prompts, candidates=None, top: int = 0) -> ops.LogProbs:
+        """Log probabilities of the token after each prompt (prompts as generate takes them, one length): of the
+        `candidates` -- the same n token ids for every prompt, or (prompts, n) of them -- with their ranks, and of the `top`
+        most likely tokens, with entropy and logsumexp (ops.LogProbs, rows in prompt order, on the GPU)."""
+        ps = [p["prompt_token_ids"] if isinstance(p, dict) else list(p) for p in prompts]
+        bs, _ = eligible_batch(ps, [SamplingParams()] * len(ps), self.max_seq)
+        ids = None if candidates is None else candidate_ids(candidates, bs, self.cfg.vocab).to(self.device)
+        return ops.logprobs(self.logits(torch.tensor(ps, dtype=torch.int32)), ids, top=top)
 
     # ------------------------------------------------------------------ vLLM-like generate
     @torch.no_grad()
@@ -198,4 +240,4 @@ class MkEngine:
 
 
 __all__ = ["MkEngine", "SamplingParams", "RequestOutput", "CompletionOutput", "NotEligible", "mk_seq_ok",
-           "eligible_batch"]
+           "eligible_batch", "candidate_ids"]

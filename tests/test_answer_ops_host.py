@@ -154,3 +154,23 @@ def test_w4_cpu_tensors():
         ops.dequantize_w4(w, dtype=torch.float16)
     with pytest.raises(_lib.MkError, match="GPU tensor"):
         ops.gemm_w4(torch.zeros(1, 64, dtype=torch.bfloat16), w)
+
+
+def test_candidate_ids():
+    from minicpm5_mk.engine import candidate_ids
+
+    assert torch.equal(candidate_ids([5, 7], 3, 10), torch.tensor([[5, 7]] * 3))
+    assert torch.equal(candidate_ids([[1, 2], [3, 4]], 2, 10), torch.tensor([[1, 2], [3, 4]]))
+    assert candidate_ids([], 2, 10).shape == (2, 0)
+    assert candidate_ids(torch.tensor([[1], [9]], dtype=torch.int32), 2, 10).dtype == torch.int64
+    for bad, msg in (([10], "token ids"), ([-1], "token ids"), ([[1], [2]], "shape"), ([[[1]]], "shape"), ([0.5], "expected"),
+                     (list(range(65)), "at most"), ([True], "expected")):
+        with pytest.raises(ValueError, match=msg):
+            candidate_ids(bad, 3, 10 if len(bad) < 65 else 100)
+
+
+def test_engine_head_option():
+    from minicpm5_mk.engine import MkEngine
+
+    with pytest.raises(ValueError, match="lm_head_quant"):
+        MkEngine("tiny", lm_head_quant="w3", log=lambda *a: None)
