@@ -291,8 +291,8 @@ int mk_lm_head_logprobs(const void* hidden, const void* weight, int T, int H, in
  * mk_gemm_w4: out (M, N) = x (M, K) (c s)^T, x bf16 at row stride ldx, f32 accumulation, out bf16 or f32 at row stride
  *   ldo; made for few rows (the weights are read once per 64 of them).  |x| up to 2^110: the codes are multiplied with an
  *   offset that is taken off again.  A row of x with an infinity or a NaN, and a weight row with a NaN scale, give NaN.
- * N, K >= 1, M >= 0; any alignment and stride of whole elements for W, x and out.  Results do not depend on timing; a
- * row's result does not depend on the other rows. */
+ * N, K >= 1, 0 <= M <= 2^19; any alignment and stride of whole elements for W, x and out.  Results do not depend on timing; a
+ * row's result does not depend on the other rows or their number. */
 int mk_w4_bytes(int N, int K, int group, size_t* codes, size_t* scales);
 int mk_w4_quantize(const void* w, size_t ldw, int N, int K, int group, void* codes, void* scales, void* stream);
 int mk_w4_dequantize(const void* codes, const void* scales, int N, int K, int group, void* out, int out_f32, size_t ldo,

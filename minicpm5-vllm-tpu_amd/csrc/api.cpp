@@ -440,7 +440,7 @@ int mk_gemm_w4(const void* x, size_t ldx, const void* codes, const void* scales,
                int out_f32, size_t ldo, void* stream) {
   int rc = w4_validate("gemm_w4", N, K, group);
   if (rc) return rc;
-  MK_REQUIRE(M >= 0, "gemm_w4: negative M");
+  MK_REQUIRE(M >= 0 && M <= (1 << 19), "gemm_w4: M must be in 0 .. 2^19");
   if (M == 0) return MK_OK;
   rc = w4_buffers("gemm_w4", codes, scales);
   if (rc) return rc;

@@ -154,13 +154,26 @@ inline LogprobPlan logprob_plan(int T, int V) {
   return {most < room ? most : room, 16};
 }
 
-// How the 4-bit product divides nrb blocks of 16 weight rows: r blocks a wave, K dealt to kw of a workgroup's 8 waves.
-struct W4Plan { int r, kw; };
-inline W4Plan w4_plan(long nrb, int nkb) {
-  if (nrb >= 16 * 256) return {2, 1};
-  int kw = 1;
-  while (kw < 8 && nrb * kw < 8 * 256 && kw * 2 <= nkb) kw *= 2;
-  return {1, kw};
+// How the 4-bit product divides M rows of x and nrb blocks of 16 weight rows, nkb blocks of 128 values of K: 16 mg rows of
+// x a workgroup, r weight blocks a wave, K dealt to kw of its waves, x staged bpc blocks of K at a time.  What orders an
+// output's sums (kw) does not depend on M: a row's result is the same in every batch.
+// Many weight rows: two blocks a wave, which halve the LDS reads of x (N = 130560, K = 1536, us, one block then two: 1 row
+// 24.0, 22.3, 16 rows 32.0, 27.2).  Fewer: K is dealt out until there are 2048 waves (M = 1, K = 8192, N = 12288, us with
+// 512, 1024, 2048, 4096 of them 36.1, 21.9, 17.2, 18.4; K = 1536, N = 9216 6.9, 5.2, 5.1, 6.3).  Up to 64 rows of x share a
+// pass over the weights, with 16 waves and twice the LDS beyond 16 (N = 130560, K = 2048, 40 rows: 8 waves 56, 16 waves
+// 50), but over a few hundred weight blocks they are shared out by 16, which fills more CUs (us, shared out then one pass:
+// N = 1536, K = 4608, 64 rows 19.4, 30.6; N = 4096, K = 4096, 40 rows 17.2, 20.1; N = 12288, K = 2048, 64 rows 23.4, 17.3).
+struct W4Plan { int mg, r, kw, bpc; };
+inline W4Plan w4_plan(int M, long nrb, int nkb) {
+  W4Plan p{1, 1, 1, 0};
+  if (nrb >= 16 * 256) p.r = 2;
+  else while (p.kw < 8 && nrb * p.kw < 8 * 256 && p.kw * 2 <= nkb) p.kw *= 2;
+  if (nrb >= 400) p.mg = M >= 64 ? 4 : (M + 15) / 16;
+  // 64 KB of x, 128 KB with more than 16 rows; whole blocks, in chunks of one size and a multiple of kw
+  const int rows = p.mg == 1 && M < 16 ? M : 16 * p.mg;
+  const int fits = (p.mg == 1 ? 256 : 512) / rows / p.kw * p.kw, chunks = (nkb + fits - 1) / fits;
+  p.bpc = ((nkb + chunks - 1) / chunks + p.kw - 1) / p.kw * p.kw;
+  return p;
 }
 
 // GEMM tile (256 of the vocabulary x 128, 192, 256 or 320 tokens) of the LM head product that keeps statistics only:

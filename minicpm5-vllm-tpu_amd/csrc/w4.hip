@@ -23,7 +23,7 @@ namespace {
 constexpr int W4_ROWS = 16, W4_K = 128;
 
 // ------------------------------------------------------------------------------------------------ quantisation
-// Bytes bound it (2 read, 1/2 written a value).  A wave makes blocks of 16 rows x 128 values: lane l reads the four
+// Bytes bound both directions (2 read and 1/2 written a value, and back): the 130560 x 1536 head 98 us each, 5.1 TB/s.  A wave makes blocks of 16 rows x 128 values: lane l reads the four
 // 16-byte pieces of row l % 16 that its 16 bytes of codes come from.
 typedef uint16_t h8 __attribute__((ext_vector_type(8), aligned(2)));
 
@@ -147,39 +147,46 @@ __global__ __launch_bounds__(256) void w4_dequantize_kernel(const uint8_t* __res
 }
 
 // ------------------------------------------------------------------------------------------------ product
-// y (M, N) = x (M, K) (c s)^T, M <= 64, f32 accumulation.  The weight stream is the bound; what it costs beside is the
-// unpacking, one VALU operation a value and lane.
+// y (M, N) = x (M, K) (c s)^T, f32 accumulation.  For few rows the weight stream is the bound: the 130560 x 1536 head takes
+// 22.3 us for one row (4.65 TB/s, what a large copy reaches), 27 for 16.  Beyond, a block of 16 x 128 weights costs a wave
+// 32 VALU operations of unpacking, and per group and 16 rows of x four to start, four to scale the accumulators and two or
+// more MFMAs, which no longer hide behind the stream: 48 rows 38.7 us, 64 rows 51.2 (K = 2048: 40 rows 48, 64 rows 56).
+// Small weights are bound by latency, one pass of loads after another (1536 x 4608, one row 5.3 us).
 //
 // A code becomes the bf16 number 16 + u = c + 24: 0x4180 with u in the mantissa, exact.  The 24 too much are taken off
 // before they are added: the accumulators of a group start at -24 sum x over the group (f32), so a group's sum is
 // sum c x, with roundings relative to 24 |sum x| at most; it is scaled by s (f32) into the row's total.
 //
-// x is staged chunk by chunk of KC values in LDS (zeros past K; rows past M hold anything: an MFMA's columns do not mix and
-// theirs are not stored), 16-byte piece p of row m at p ^ (m % 16) so that
-// the 16 rows of an operand read are on distinct banks; its group sums are made on the way.  A workgroup has 8 waves:
-// 8 / KW sets of R row blocks, each set's K blocks dealt to KW waves, whose totals are added in wave order at the end.
-constexpr int W4_WAVES = 8, W4_TH = 64 * W4_WAVES;
+// x is staged in LDS, as many blocks of 128 values of K at a time as fit (zeros past K), each block its rows of 256 bytes,
+// 16-byte piece p of row m at p ^ (m % 16) so that the 16 rows of an operand read are on distinct banks; its group sums are
+// made on the way.  MFMA columns past the rows hold whatever lies there, columns do not mix and theirs are not stored.  A
+// workgroup's waves are sets of kw: a set has R row blocks, whose K blocks are dealt to its waves, their totals added in
+// wave order at the end.  A wave loads the next of its blocks while it multiplies one.
+constexpr int w4_waves(int mg) { return mg == 1 ? 8 : 16; }
+constexpr int w4_xb(int mg) { return w4_waves(mg) * 8192; }   // LDS bytes of x, and of its sums (groups of 32)
+constexpr int w4_sb(int mg) { return w4_xb(mg) / 16; }
 
 __device__ inline uint32_t pair_bf16(uint32_t w, int p) {
   const uint32_t v = p == 0 ? w << 3 : w >> (4 * p - 3);
   return (v & 0x00780078u) | 0x41804180u;
 }
 
-template <int MG>
-constexpr int w4_kc() { return MG == 1 ? 1024 : MG == 2 ? 1024 : 512; }   // values of K per chunk
-
 template <int MG, int R, int GROUP>
-__global__ __launch_bounds__(W4_TH) void w4_gemm_kernel(W4GemmArgs a, int nkb, int kw) {
-  constexpr int KC = w4_kc<MG>(), BPC = KC / W4_K, GPB = W4_K / GROUP, GPC = KC / GROUP, ROWS = 16 * MG;
-  constexpr int XB = ROWS * KC * 2, SB = GPC * ROWS * 4;
-  constexpr int RED = W4_WAVES * R * MG * 64 * 16;   // totals of every wave
-  __shared__ __attribute__((aligned(16))) char smem[XB + SB > RED ? XB + SB : RED];
+__global__ __launch_bounds__(64 * w4_waves(MG), 4) void w4_gemm_kernel(W4GemmArgs a, int nkb, int kw, int bpc) {
+  constexpr int W4_WAVES = w4_waves(MG), W4_TH = 64 * W4_WAVES, W4_XB = w4_xb(MG), W4_SB = w4_sb(MG);
+  constexpr int GPB = W4_K / GROUP, ROWS = 16 * MG;
+  static_assert(R > 1 || W4_WAVES * MG * 64 * 16 <= W4_XB, "the totals of a dealt K fit where x was");
+  __shared__ __attribute__((aligned(16))) char smem[W4_XB + W4_SB];
   const int lane = threadIdx.x & 63, c16 = lane & 15, kq = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kwi = w % kw;
+  const int mrow0 = blockIdx.y * ROWS, M = std::min(ROWS, a.M - mrow0);
+  const uint16_t* x = a.x + (size_t)mrow0 * a.ldx;
   const long nrb = (a.N + W4_ROWS - 1) / W4_ROWS;
   const long rb0 = ((long)blockIdx.x * (W4_WAVES / kw) + w / kw) * R;
-  float* sums = reinterpret_cast<float*>(smem + XB);
+  float* sums = reinterpret_cast<float*>(smem + W4_XB);
+  const int ppr = bpc * 16;                   // 16-byte pieces of a staged row
+  const int RA = MG == 1 ? M : ROWS;          // rows of a staged block
 
   f32x4 tot[R][MG];
 #pragma unroll
@@ -198,33 +205,50 @@ __global__ __launch_bounds__(W4_TH) void w4_gemm_kernel(W4GemmArgs a, int nkb, i
       sc[r] = *reinterpret_cast<const SC*>(a.scales + b * W4_ROWS * GPB + kq * 4 * GPB);
     }
   };
-  int kb = kwi;
-  if (kb < nkb) load(kb);
-  for (int c0 = 0; c0 < nkb; c0 += BPC) {
-    __syncthreads();   // the last chunk's operand reads are done
-    // stage x: thread -> (row, 16-byte piece), the pieces of a row on consecutive lanes
-    for (int i = threadIdx.x; i < a.M * (KC / 8); i += W4_TH) {
-      const int m = i / (KC / 8), p = i % (KC / 8), k = c0 * W4_K + 8 * p;
-      h8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-      const uint16_t* xr = a.x + (size_t)m * a.ldx;
-      if (k + 8 <= a.K) {
-        v = *reinterpret_cast<const h8*>(xr + k);
-      } else {
+  // this lane's operand row (of every 16) and its piece of k-step t in a staged block
+  const int xrow = MG == 1 ? std::min(c16, M - 1) : c16;
+  int xoff[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (k + e < a.K) v[e] = xr[k + e];
+  for (int t = 0; t < 4; ++t) xoff[t] = xrow * 256 + (((4 * t + kq) ^ xrow) & 15) * 16;
+  if (kwi < nkb) load(kwi);
+
+  for (int c0 = 0; c0 < nkb; c0 += bpc) {
+    if (c0) __syncthreads();   // the last chunk's operand reads are done
+    // stage x: thread -> (row, 16-byte piece), the pieces of a row on consecutive lanes, four of a thread's loads on the way
+    // together
+    for (int i0 = threadIdx.x; i0 < M * ppr; i0 += 4 * W4_TH) {
+      h8 v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = i0 + q * W4_TH, m = i / ppr, k = c0 * W4_K + 8 * (i - m * ppr);
+        v[q] = h8{0, 0, 0, 0, 0, 0, 0, 0};
+        if (m >= M) continue;
+        const uint16_t* xr = x + (size_t)m * a.ldx;
+        if (k + 8 <= a.K) {
+          v[q] = *reinterpret_cast<const h8*>(xr + k);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (k + e < a.K) v[q][e] = xr[k + e];
+        }
       }
-      *reinterpret_cast<u32x4*>(smem + (m * (KC / 8) + (p ^ (m & 15))) * 16) = __builtin_bit_cast(u32x4, v);
-      float s = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += bf2f(v[e]);
+      for (int q = 0; q < 4; ++q) {
+        const int i = i0 + q * W4_TH, m = i / ppr, p = i - m * ppr;
+        if (m >= M) break;
+        *reinterpret_cast<u32x4*>(smem + ((p >> 4) * RA + m) * 256 + ((p ^ m) & 15) * 16) = __builtin_bit_cast(u32x4, v[q]);
+        float s = 0.f;
 #pragma unroll
-      for (int o = 1; o < GROUP / 8; o <<= 1) s += __shfl_xor(s, o);
-      if (p % (GROUP / 8) == 0) sums[(p / (GROUP / 8)) * ROWS + m] = -24.f * s;
+        for (int e = 0; e < 8; ++e) s += bf2f(v[q][e]);
+#pragma unroll
+        for (int o = 1; o < GROUP / 8; o <<= 1) s += __shfl_xor(s, o);   // ppr is a multiple of 16: whole groups
+        if (p % (GROUP / 8) == 0) sums[(p / (GROUP / 8)) * RA + m] = -24.f * s;
+      }
     }
     __syncthreads();
-    const int ce = std::min(c0 + BPC, nkb);
-    for (; kb < ce; kb += kw) {
+    const int ce = std::min(c0 + bpc, nkb);
+    for (int kb = c0 + kwi; kb < ce; kb += kw) {
+      const int lb = kb - c0;   // block of the chunk
       u32x4 cb[R];
       SC sb[R];
 #pragma unroll
@@ -233,13 +257,12 @@ __global__ __launch_bounds__(W4_TH) void w4_gemm_kernel(W4GemmArgs a, int nkb, i
         sb[r] = sc[r];
       }
       if (kb + kw < nkb) load(kb + kw);
-      const int lb = kb - c0;   // block of the chunk
 #pragma unroll
       for (int g = 0; g < GPB; ++g) {
         f32x4 acc[R][MG];
 #pragma unroll
         for (int m = 0; m < MG; ++m) {
-          const float z = sums[(lb * GPB + g) * ROWS + 16 * m + c16];
+          const float z = sums[(lb * GPB + g) * RA + 16 * m + xrow];
 #pragma unroll
           for (int r = 0; r < R; ++r) acc[r][m] = f32x4{z, z, z, z};
         }
@@ -252,11 +275,11 @@ __global__ __launch_bounds__(W4_TH) void w4_gemm_kernel(W4GemmArgs a, int nkb, i
             for (int p = 0; p < 4; ++p) av[r][p] = pair_bf16(cb[r][t], p);
 #pragma unroll
           for (int m = 0; m < MG; ++m) {
-            const u32x4 bv = *reinterpret_cast<const u32x4*>(
-                smem + ((16 * m + c16) * (KC / 8) + ((lb * 16 + 4 * t + kq) ^ c16)) * 16);
+            const u32x4 bv = *reinterpret_cast<const u32x4*>(smem + lb * RA * 256 + xoff[t] + m * 4096);
 #pragma unroll
             for (int r = 0; r < R; ++r) acc[r][m] = mfma_bf16_16x16x32(av[r], bv, acc[r][m]);
           }
+          if constexpr (MG * R >= 4) __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -295,8 +318,8 @@ __global__ __launch_bounds__(W4_TH) void w4_gemm_kernel(W4GemmArgs a, int nkb, i
     if (n >= a.N) continue;
 #pragma unroll
     for (int m = 0; m < MG; ++m) {
-      const int row = 16 * m + c16;
-      if (row >= a.M) continue;
+      if (16 * m + c16 >= M) continue;
+      const int row = mrow0 + 16 * m + c16;
       const f32x4 v = tot[r][m];
       if (a.out_f32) {
         float* o = static_cast<float*>(a.out) + (size_t)row * a.ldo + n;
@@ -316,38 +339,37 @@ __global__ __launch_bounds__(W4_TH) void w4_gemm_kernel(W4GemmArgs a, int nkb, i
 }
 
 template <int MG, int R>
-void launch_group(const W4GemmArgs& a, int nkb, int kw, unsigned grid, hipStream_t st) {
+void launch_tile(const W4GemmArgs& a, int nkb, int kw, int bpc, hipStream_t st) {
+  const long nrb = (a.N + W4_ROWS - 1) / W4_ROWS, per = (long)w4_waves(MG) / kw * R;
+  const dim3 grid((unsigned)((nrb + per - 1) / per), (a.M + 16 * MG - 1) / (16 * MG)), block(64 * w4_waves(MG));
   switch (a.group) {
-    case 32: hipLaunchKernelGGL((w4_gemm_kernel<MG, R, 32>), dim3(grid), dim3(W4_TH), 0, st, a, nkb, kw); break;
-    case 64: hipLaunchKernelGGL((w4_gemm_kernel<MG, R, 64>), dim3(grid), dim3(W4_TH), 0, st, a, nkb, kw); break;
-    default: hipLaunchKernelGGL((w4_gemm_kernel<MG, R, 128>), dim3(grid), dim3(W4_TH), 0, st, a, nkb, kw); break;
+    case 32: hipLaunchKernelGGL((w4_gemm_kernel<MG, R, 32>), grid, block, 0, st, a, nkb, kw, bpc); break;
+    case 64: hipLaunchKernelGGL((w4_gemm_kernel<MG, R, 64>), grid, block, 0, st, a, nkb, kw, bpc); break;
+    default: hipLaunchKernelGGL((w4_gemm_kernel<MG, R, 128>), grid, block, 0, st, a, nkb, kw, bpc); break;
   }
-}
-
-template <int MG>
-void launch_rows(const W4GemmArgs& a, hipStream_t st) {
-  const int nkb = (a.K + W4_K - 1) / W4_K;
-  const long nrb = (a.N + W4_ROWS - 1) / W4_ROWS;
-  const W4Plan pl = w4_plan(nrb, nkb);
-  const long per = (long)W4_WAVES / pl.kw * pl.r;
-  const unsigned grid = (unsigned)((nrb + per - 1) / per);
-  if (pl.r == 2) launch_group<MG, 2>(a, nkb, pl.kw, grid, st);
-  else launch_group<MG, 1>(a, nkb, pl.kw, grid, st);
 }
 
 }  // namespace
 
-int launch_w4_gemm(const W4GemmArgs& a0, hipStream_t st) {
-  for (int m0 = 0; m0 < a0.M; m0 += 64) {
-    W4GemmArgs a = a0;
-    a.M = std::min(64, a0.M - m0);
-    a.x = a0.x + (size_t)m0 * a0.ldx;
-    a.out = static_cast<char*>(a0.out) + (size_t)m0 * a0.ldo * (a0.out_f32 ? 4 : 2);
-    if (a.M <= 16) launch_rows<1>(a, st);
-    else if (a.M <= 32) launch_rows<2>(a, st);
-    else launch_rows<4>(a, st);
-    MK_HIP_CHECK(hipGetLastError());
+int launch_w4_gemm(const W4GemmArgs& a, hipStream_t st) {
+  const int nkb = (a.K + W4_K - 1) / W4_K;
+  const W4Plan pl = w4_plan(a.M, (a.N + W4_ROWS - 1) / W4_ROWS, nkb);
+  if (pl.r == 1) {
+    switch (pl.mg) {
+      case 1: launch_tile<1, 1>(a, nkb, pl.kw, pl.bpc, st); break;
+      case 2: launch_tile<2, 1>(a, nkb, pl.kw, pl.bpc, st); break;
+      case 3: launch_tile<3, 1>(a, nkb, pl.kw, pl.bpc, st); break;
+      default: launch_tile<4, 1>(a, nkb, pl.kw, pl.bpc, st); break;
+    }
+  } else {
+    switch (pl.mg) {
+      case 1: launch_tile<1, 2>(a, nkb, pl.kw, pl.bpc, st); break;
+      case 2: launch_tile<2, 2>(a, nkb, pl.kw, pl.bpc, st); break;
+      case 3: launch_tile<3, 2>(a, nkb, pl.kw, pl.bpc, st); break;
+      default: launch_tile<4, 2>(a, nkb, pl.kw, pl.bpc, st); break;
+    }
   }
+  MK_HIP_CHECK(hipGetLastError());
   return MK_OK;
 }
 

@@ -118,7 +118,8 @@ def _w4(name, **kw):
     ("quantize", dict(ldw=255), -1, "stride"),
     ("dequantize", dict(out=BOGUS + 2, f32=1), -1, "misaligned"),
     ("dequantize", dict(ldo=255), -1, "stride"),
-    ("gemm", dict(M=-1), -1, "negative"),
+    ("gemm", dict(M=-1), -1, "M must be"),
+    ("gemm", dict(M=(1 << 19) + 1), -1, "M must be"),
     ("gemm", dict(x=None), -1, "null"),
     ("gemm", dict(x=BOGUS + 1), -1, "misaligned"),
     ("gemm", dict(ldx=255), -1, "stride"),

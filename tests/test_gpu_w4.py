@@ -129,14 +129,16 @@ def test_gemm(m, n, k, group):
 
 
 def test_gemm_rows_alone():
-    """A row's result does not depend on the other rows of its group of 16."""
+    """A row's result does not depend on the other rows or how many they are: one block or several a wave, K dealt out or
+    not."""
     from minicpm5_mk import ops
 
-    q = ops.quantize_w4(_weight(300, 700), 64)
-    x = _x(16, 700)
-    full = ops.gemm_w4(x, q, dtype=F32)
-    for i in (0, 7, 15):
-        assert torch.equal(ops.gemm_w4(x[i:i + 1], q, dtype=F32), full[i:i + 1])
+    for n, k in ((300, 700), (7000, 2300), (66000, 300)):
+        q = ops.quantize_w4(_weight(n, k), 64)
+        x = _x(150, k)
+        full = ops.gemm_w4(x, q, dtype=F32)
+        for m0, m1 in ((0, 1), (7, 8), (3, 19), (20, 53), (60, 124), (149, 150)):
+            assert torch.equal(ops.gemm_w4(x[m0:m1], q, dtype=F32), full[m0:m1]), (n, m0, m1)
 
 
 def test_gemm_strides():
