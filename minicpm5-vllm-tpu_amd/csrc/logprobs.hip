@@ -374,21 +374,31 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 6) void logprob_rows_
       // its tile passes the last one.  Other waves' entries may be older: lower, still bounds.
       lmax = fmaxf(lmax, tm);
       if (first) {
-        top.bound(kth_bound(tm, a.top), c1);   // where less than k groups have a value
+        // where less than k groups may have a value: the wave's own lanes
+        if (c1 - c0 < WAVES * LP_TILE) top.bound(kth_bound(tm, a.top), c1);
         publish();
         __syncthreads();
       }
       if (__ballot(top.may_pass(tm, t0))) {
         if (!first) publish();
         top.bound(kth_bound(*const_cast<volatile float*>(&sh.gmax[lane]), a.top), c1);
-        uint32_t some = 0;                 // the lane's values that may pass; few, and read again: v has no index
+        // The lane's values that may pass: mostly one, its largest (the first of equals); any others are read again, as v
+        // has no index.
+        uint32_t some = 0, best = 1u << LP_E;
 #pragma unroll
-        for (int e = 0; e < LP_E; ++e) some |= (uint32_t)top.may_pass(v[e], t0) << e;
+        for (int e = LP_E - 1; e >= 0; --e) {
+          some |= (uint32_t)top.may_pass(v[e], t0) << e;
+          best = v[e] == tm ? 1u << e : best;
+        }
+        float cv = tm;
+        uint32_t bit = some & best;
         while (__ballot(some)) {
-          const int i = at(t0, __builtin_ctz(some | 1u << LP_E));
-          const bool have = some && i < c1;
-          top.offer(have, have ? L::f(x[i]) : 0.f, i);
-          some &= some - 1;
+          const int i = at(t0, __builtin_ctz(bit | 1u << LP_E));
+          top.offer(bit && i < c1, cv, i);
+          some &= ~bit;
+          bit = some & (0u - some);
+          const int next = at(t0, __builtin_ctz(bit | 1u << LP_E));
+          if (bit && next < c1) cv = L::f(x[next]);
         }
       }
     }

@@ -143,15 +143,16 @@ inline bool lm_head_skinny(int rows, int V, int K) {
 // 203, 16 288; V = 8000, 4096 rows 41, 58, 122).  Rows for one or two workgroups a CU: more waves each (bf16 V = 130560,
 // 500 rows 52, 40, 46; 700 rows 60, 52, 65; f32 1000 rows 107, 114, 114; 200 rows 72, 48, 35).  Few long rows are split,
 // as the exponentials of a 130560-value row alone take one CU 12 us; that costs a second launch (f32 V = 130560, one
-// then split: 1 row 24.0, 13.1, 33 rows 36.3, 24.8, 65 rows 29.7, 22.6, 200 rows in two 34.7, 46.5; 8 rows of 65536
-// 17.3, 13.5).
+// then split: 1 row 24.0, 13.5, 33 rows 36.3, 21.5, 65 rows 29.7, 22.3, 200 rows in two 34.7, 46.5; 8 rows of 65536
+// 17.3, 13.1); the splits are of one size, whole rounds of 16 tiles.
 struct LogprobPlan { int splits, waves; };
 inline LogprobPlan logprob_plan(int T, int V) {
   if (T > 896) return {1, 4};
   if (T > 256) return {1, 8};
-  const int most = ((V + 1023) / 1024 + 15) / 16, room = T > 0 ? 256 / T : 1;
+  const int tiles = (V + 1023) / 1024, most = (tiles + 15) / 16, room = T > 0 ? 256 / T : 1;
   if (most <= 2 || room <= 1) return {1, 16};
-  return {most < room ? most : room, 16};
+  const int rounds = (most + room - 1) / room;   // of 16 tiles a workgroup
+  return {(tiles + 16 * rounds - 1) / (16 * rounds), 16};
 }
 
 // How the 4-bit product divides M rows of x and nrb blocks of 16 weight rows, nkb blocks of 128 values of K: 16 mg rows of

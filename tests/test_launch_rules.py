@@ -163,7 +163,7 @@ def test_logprob_plan(rules):
             splits, waves = _ints(rules.logprob_plan, 2, T, V)
             assert waves in (4, 8, 16) and splits >= 1
             assert splits == 1 or (waves == 16 and T * splits <= 256 and splits <= -(-V // 16384))
-    assert _ints(rules.logprob_plan, 2, 1, 130560) == (8, 16) and _ints(rules.logprob_plan, 2, 33, 130560) == (7, 16)
+    assert _ints(rules.logprob_plan, 2, 1, 130560) == (8, 16) and _ints(rules.logprob_plan, 2, 33, 130560) == (4, 16)
     assert _ints(rules.logprob_plan, 2, 200, 130560) == (1, 16) and _ints(rules.logprob_plan, 2, 500, 130560) == (1, 8)
     assert _ints(rules.logprob_plan, 2, 2048, 130560) == (1, 4)
 
