@@ -530,52 +530,25 @@ int launch_t(const LogprobArgs& a, void* ws, hipStream_t st) {
 }
 
 // ------------------------------------------------------------------------------------------------ from hidden states
-// The rows' log probabilities from the statistics the LM head product leaves (launch_gemm_lse): a workgroup merges 16 rows'
-// `tiles` entries, 16 threads a row, and makes the given tokens' logits as dot products of f32 sums, a wave each.
-constexpr int HF_ROWS = 16, HF_PARTS = 16;
+// The rows' log probabilities from the statistics the LM head product leaves (launch_gemm_lse): a workgroup has 32 rows,
+// whole cache lines of the statistics.  Its waves first make the given tokens' logits, dot products of f32 sums, a wave
+// each; then 32 threads a row merge its `tiles` entries.
+constexpr int HF_ROWS = 32, HF_WAVES = 16, HF_PARTS = 64 * HF_WAVES / HF_ROWS;
 
-__global__ __launch_bounds__(256) void head_finish_kernel(HeadLogprobArgs a, int tiles, const float* part) {
-  __shared__ float sh[3][HF_PARTS][HF_ROWS];
+__global__ __launch_bounds__(64 * HF_WAVES) void head_finish_kernel(HeadLogprobArgs a, int tiles, const float* part) {
+  __shared__ float sh[3][HF_WAVES][HF_ROWS];
+  __shared__ float dot[HF_ROWS * LP_MAX_IDS];
   __shared__ double lse[HF_ROWS];
   const int r = threadIdx.x % HF_ROWS, q = threadIdx.x / HF_ROWS, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int row0 = blockIdx.x * HF_ROWS, row = row0 + r;
-  // log2 units: m a reference exponent, as the tiles' are
-  float m = NEG_MAX, s = 0.f, u = 0.f;
-  auto merge = [&](float m2, float s2, float u2) {
-    const float mn = fmaxf(m, m2), d1 = fmaxf(m - mn, -1e4f), d2 = fmaxf(m2 - mn, -1e4f);
-    const float f1 = fast_exp2(d1), f2 = fast_exp2(d2);
-    u = f1 * fmaf(d1, s, u) + f2 * fmaf(d2, s2, u2);
-    s = f1 * s + f2 * s2;
-    m = mn;
+  const int row0 = blockIdx.x * HF_ROWS, row = row0 + r, given = min(HF_ROWS, a.T - row0) * a.n_ids;
+  auto id_of = [&](int i) {
+    const size_t o = (size_t)row0 * a.n_ids + i;
+    return a.ids64 ? static_cast<const long long*>(a.ids)[o] : static_cast<const int*>(a.ids)[o];
   };
-  const float* p = part + min(row, a.T - 1);
-#pragma unroll 4
-  for (int t = q; t < tiles; t += HF_PARTS) {
-    const float* e = p + (size_t)t * 3 * a.T;
-    merge(e[0], e[a.T], e[2 * (size_t)a.T]);
-  }
-  sh[0][q][r] = m;
-  sh[1][q][r] = s;
-  sh[2][q][r] = u;
-  __syncthreads();
-  if (q == 0) {
-#pragma unroll
-    for (int o = 1; o < HF_PARTS; ++o) merge(sh[0][o][r], sh[1][o][r], sh[2][o][r]);
-    const double ln2 = 0.6931471805599453, l2 = (double)log2f(s);
-    lse[r] = ((double)m + l2) * ln2;
-    if (row < a.T) {
-      a.lse[row] = (float)lse[r];
-      a.entropy[row] = (float)((l2 - (double)(u / s)) * ln2);
-    }
-  }
-  __syncthreads();
-  for (int i = w; i < HF_ROWS * a.n_ids; i += 4) {
-    const int rr = row0 + i / a.n_ids;
-    if (rr >= a.T) break;
-    const size_t o = (size_t)rr * a.n_ids + i % a.n_ids;
-    const long long id = a.ids64 ? static_cast<const long long*>(a.ids)[o] : static_cast<const int*>(a.ids)[o];
+  for (int i = w; i < given; i += HF_WAVES) {
+    const long long id = id_of(i);
     const bool in = id >= 0 && id < a.V;
-    const uint16_t *h = a.hidden + (size_t)rr * a.H, *wt = a.weight + (size_t)(in ? id : 0) * a.H;
+    const uint16_t *h = a.hidden + (size_t)(row0 + i / a.n_ids) * a.H, *wt = a.weight + (size_t)(in ? id : 0) * a.H;
     float d = 0.f;
     for (int k = lane * 8; k < a.H; k += 512) {
       const u32x4 hv = *reinterpret_cast<const u32x4*>(h + k), wv = *reinterpret_cast<const u32x4*>(wt + k);
@@ -586,9 +559,48 @@ __global__ __launch_bounds__(256) void head_finish_kernel(HeadLogprobArgs a, int
       }
     }
     d = wave_sum(d);
-    const double l = lse[rr - row0];
+    if (lane == 0) dot[i] = d;
+  }
+  // log2 units: m a reference exponent, as the tiles' are
+  float m = NEG_MAX, s = 0.f, u = 0.f;
+  auto merge = [&](float m2, float s2, float u2) {
+    const float mn = fmaxf(m, m2), d1 = fmaxf(m - mn, -1e4f), d2 = fmaxf(m2 - mn, -1e4f);
+    const float f1 = fast_exp2(d1), f2 = fast_exp2(d2);
+    u = f1 * fmaf(d1, s, u) + f2 * fmaf(d2, s2, u2);
+    s = f1 * s + f2 * s2;
+    m = mn;
+  };
+  const float* p = part + min(row, a.T - 1);
+#pragma unroll 8
+  for (int t = q; t < tiles; t += HF_PARTS) {
+    const float* e = p + (size_t)t * 3 * a.T;
+    merge(e[0], e[a.T], e[2 * (size_t)a.T]);
+  }
+#pragma unroll
+  for (int o = HF_ROWS; o <= 32; o <<= 1) merge(__shfl_xor(m, o), __shfl_xor(s, o), __shfl_xor(u, o));
+  if (lane < HF_ROWS) {
+    sh[0][w][r] = m;
+    sh[1][w][r] = s;
+    sh[2][w][r] = u;
+  }
+  __syncthreads();
+  if (q == 0) {
+#pragma unroll
+    for (int o = 1; o < HF_WAVES; ++o) merge(sh[0][o][r], sh[1][o][r], sh[2][o][r]);
+    const double ln2 = 0.6931471805599453, l2 = (double)log2f(s);
+    lse[r] = ((double)m + l2) * ln2;
+    if (row < a.T) {
+      a.lse[row] = (float)lse[r];
+      a.entropy[row] = (float)((l2 - (double)(u / s)) * ln2);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < given; i += 64 * HF_WAVES) {
+    const long long id = id_of(i);
+    const double l = lse[i / a.n_ids];
     // a NaN row is NaN for every id; rounding may put a certain token a step above 0
-    if (lane == 0) a.token_lp[o] = !(l == l) ? __builtin_nanf("") : in ? fminf((float)((double)d - l), 0.f) : neg_inf();
+    a.token_lp[(size_t)row0 * a.n_ids + i] =
+        !(l == l) ? __builtin_nanf("") : id >= 0 && id < a.V ? fminf((float)((double)dot[i] - l), 0.f) : neg_inf();
   }
 }
 
@@ -662,7 +674,7 @@ int launch_head_logprobs(const HeadLogprobArgs& a, void* ws, hipStream_t st) {
       const int rc = launch_gemm_lse(g, st);
       if (rc) return rc;
     }
-    hipLaunchKernelGGL(head_finish_kernel, dim3((h.T + HF_ROWS - 1) / HF_ROWS), dim3(256), 0, st, h, tiles,
+    hipLaunchKernelGGL(head_finish_kernel, dim3((h.T + HF_ROWS - 1) / HF_ROWS), dim3(64 * HF_WAVES), 0, st, h, tiles,
                        static_cast<const float*>(ws));
     MK_HIP_CHECK(hipGetLastError());
   }
