@@ -1802,6 +1802,10 @@ int launch_gemm_lse(const GemmArgs& g0, hipStream_t st) {
   if (rc) return rc;
   MK_REQUIRE(g.K % 32 == 0 && g.ldo >= g.N, "gemm_lse: K must be a multiple of 32 and ldo at least N");
   static_assert(CfgM::BM == LSE_ROWS && CfgN::BM == LSE_ROWS && CfgX::BM == LSE_ROWS && CfgW4::BM == LSE_ROWS, "one statistic per 256 rows, whatever the tile");
+  // tile-order groups of 6 x 256 of the vocabulary: an XCD's 32 tiles at a time are then 6 weight and 5 - 6 token panels
+  // (us against the common rule, which is made for few weight panels: 8192 rows of the 1b head 2641, 2602, 4096 of the 2b
+  // head 1671, 1655, 1000 of the 1b head 352, 347)
+  g.gm = 6;
   switch (lse_tile(g.N)) {
     case 2: launch_c<CfgM, GemmIn::BF16, Epi::LSE>(g, st); break;
     case 5: launch_c<CfgN, GemmIn::BF16, Epi::LSE>(g, st); break;
