@@ -6,9 +6,8 @@ kernels.  Each wrapper checks dtypes, devices, contiguity and shapes on the host
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
-from dataclasses import dataclass
+import functools
 from typing import NamedTuple
 
 import torch
@@ -16,7 +15,7 @@ import torch
 from . import _lib
 from ._lib import EPI, MkError, check, load
 
-BF16 = torch.bfloat16
+BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
 
 
 def _stream():
@@ -43,17 +42,21 @@ def _need(t: torch.Tensor, name: str, dtype=None, shape=None):
 
 
 def _need_rows(t: torch.Tensor, name: str, dtypes, cols: int | None = None):
-    """A (rows, cols) GPU tensor of one of `dtypes` whose rows are contiguous, at any row stride and alignment."""
+    """A (rows, cols) GPU tensor of one of `dtypes` whose rows are contiguous, at any row stride and alignment ->
+    (rows, cols, row stride)."""
     if not isinstance(t, torch.Tensor):
         raise MkError(f"{name}: expected a torch.Tensor")
     if not t.is_cuda:
         raise MkError(f"{name}: must be a GPU tensor (libmk has no CPU path)")
-    if t.dim() != 2 or t.dtype not in dtypes:
+    if t.ndim != 2 or t.dtype not in dtypes:
         raise MkError(f"{name}: {tuple(t.shape)} {t.dtype}, expected 2 dimensions of {' / '.join(str(d) for d in dtypes)}")
-    if cols is not None and t.shape[1] != cols:
-        raise MkError(f"{name}: {t.shape[1]} columns, expected {cols}")
-    if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+    rows, c = t.shape
+    if cols is not None and c != cols:
+        raise MkError(f"{name}: {c} columns, expected {cols}")
+    s0, s1 = t.stride()
+    if (s1 != 1 and c > 1 and rows > 0) or (s0 < c and rows > 1):
         raise MkError(f"{name}: rows must be contiguous and must not overlap")
+    return rows, c, s0
 
 
 def _same_device(t: torch.Tensor, **others):
@@ -62,17 +65,17 @@ def _same_device(t: torch.Tensor, **others):
             raise MkError(f"{name}: on {o.device}, expected {t.device}")
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(t: torch.Tensor):
-    """Makes t's device the current one, so that its stream, allocations and launches are that device's."""
-    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-def _raw_stream() -> int:
-    """The current stream's handle, without the Stream object around it (2.7 us of a call)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+def _call(t: torch.Tensor, fn, what: str, *args):
+    """check(fn(*args, stream)) with t's device the current one and that device's current stream (its raw handle: a
+    Stream object around it costs 2.7 us of a call)."""
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, what)
 
 
 def _adr(t):
@@ -237,28 +240,26 @@ def logprobs(logits: torch.Tensor, ids: torch.Tensor | None = None, top: int = 0
     masked): log probabilities and logsumexp -inf, entropy 0.  A row with NaN or +inf: NaN, ranks and top_ids -1.
     Rows may be strided (a slice of a padded vocabulary).  No gradient."""
     lib = load()
-    _need_rows(logits, "logits", tuple(LOGITS_TYPES))
-    T, V = logits.shape
+    T, V, ld = _need_rows(logits, "logits", LOGITS_TYPES)
     if V < 1:
         raise MkError("logits: empty vocabulary")
     top = int(top)
     if not 0 <= top <= min(LOGPROBS_MAX, V):
         raise MkError(f"top: {top}, expected 0 .. {min(LOGPROBS_MAX, V)}")
-    n = 0 if ids is None else _need_ids(ids, T)
-    _same_device(logits, ids=ids)
-    dev, f32, i32 = logits.device, torch.float32, torch.int32
-    with _on(logits):
-        lp = rk = tl = ti = None
-        if ids is not None:
-            lp, rk = torch.empty(ids.shape, dtype=f32, device=dev), torch.empty(ids.shape, dtype=i32, device=dev)
-        if top:
-            tl, ti = torch.empty((T, top), dtype=f32, device=dev), torch.empty((T, top), dtype=i32, device=dev)
-        ent, lse = torch.empty((2, T), dtype=f32, device=dev).unbind()
-        nbytes = int(lib.mk_logprobs_scratch_bytes(T, V, n, top))
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        check(lib.mk_logprobs(_adr(logits), LOGITS_TYPES[logits.dtype], logits.stride(0), T, V, _adr(ids),
-                              int(n > 0 and ids.dtype == torch.int64), n, top, _adr(lp), _adr(rk), _adr(tl), _adr(ti),
-                              _adr(ent), _adr(lse), _adr(scratch), nbytes, _raw_stream()), "mk_logprobs")
+    n = 0
+    lp = rk = tl = ti = None
+    if ids is not None:
+        n = _need_ids(ids, T)
+        _same_device(logits, ids=ids)
+        lp, rk = logits.new_empty(ids.shape, dtype=F32), logits.new_empty(ids.shape, dtype=I32)
+    if top:
+        tl, ti = logits.new_empty((T, top), dtype=F32), logits.new_empty((T, top), dtype=I32)
+    ent, lse = logits.new_empty((2, T), dtype=F32).unbind()
+    nbytes = int(lib.mk_logprobs_scratch_bytes(T, V, n, top))
+    scratch = logits.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _call(logits, lib.mk_logprobs, "mk_logprobs", _adr(logits), LOGITS_TYPES[logits.dtype], ld, T, V, _adr(ids),
+          int(n > 0 and ids.dtype == torch.int64), n, top, _adr(lp), _adr(rk), _adr(tl), _adr(ti), _adr(ent), _adr(lse),
+          _adr(scratch), nbytes)
     return LogProbs(lp, rk, tl, ti, ent, lse)
 
 
@@ -278,20 +279,16 @@ def lm_head_logprobs(hidden: torch.Tensor, weight: torch.Tensor, ids: torch.Tens
         raise MkError("weight: empty vocabulary")
     n = 0 if ids is None else _need_ids(ids, T)
     _same_device(hidden, weight=weight, ids=ids)
-    dev = hidden.device
-    with _on(hidden):
-        lp = None if ids is None else torch.empty(ids.shape, dtype=torch.float32, device=dev)
-        ent, lse = torch.empty((2, T), dtype=torch.float32, device=dev).unbind()
-        nbytes = int(lib.mk_lm_head_logprobs_scratch_bytes(T, V, n))
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        check(lib.mk_lm_head_logprobs(_adr(hidden), _adr(weight), T, H, V, _adr(ids),
-                                      int(n > 0 and ids.dtype == torch.int64), n, _adr(lp), _adr(ent), _adr(lse),
-                                      _adr(scratch), nbytes, _raw_stream()), "mk_lm_head_logprobs")
+    lp = None if ids is None else hidden.new_empty(ids.shape, dtype=F32)
+    ent, lse = hidden.new_empty((2, T), dtype=F32).unbind()
+    nbytes = int(lib.mk_lm_head_logprobs_scratch_bytes(T, V, n))
+    scratch = hidden.new_empty(nbytes, dtype=torch.uint8)
+    _call(hidden, lib.mk_lm_head_logprobs, "mk_lm_head_logprobs", _adr(hidden), _adr(weight), T, H, V, _adr(ids),
+          int(n > 0 and ids.dtype == torch.int64), n, _adr(lp), _adr(ent), _adr(lse), _adr(scratch), nbytes)
     return LogProbs(lp, None, None, None, ent, lse)
 
 
-@dataclass(frozen=True)
-class W4Weight:
+class W4Weight(NamedTuple):
     """A weight (n, k) in 4 bits with a bf16 scale per row and `group` values of k, in libmk's block layout
     (include/mk.h, mk_w4_quantize).  Made by quantize_w4."""
     codes: torch.Tensor    # uint8
@@ -301,66 +298,72 @@ class W4Weight:
     group: int
 
 
+@functools.lru_cache(maxsize=256)
 def _w4_sizes(n: int, k: int, group: int):
+    """Bytes of the codes and the scales."""
     codes, scales = ctypes.c_size_t(), ctypes.c_size_t()
     check(load().mk_w4_bytes(n, k, group, ctypes.byref(codes), ctypes.byref(scales)), "mk_w4_bytes")
     return codes.value, scales.value
 
 
 def _need_w4(w):
+    """The kernels take a W4Weight's sizes on trust: its buffers have to be as large as those say."""
     if not isinstance(w, W4Weight):
         raise MkError("expected a W4Weight (quantize_w4)")
+    nc, ns = _w4_sizes(w.n, w.k, w.group)
+    c, s = w.codes, w.scales
+    if not c.is_cuda or s.device != c.device:
+        raise MkError("W4Weight: codes and scales must be GPU tensors of one device")
+    if c.dtype != torch.uint8 or s.dtype != BF16 or c.numel() != nc or s.numel() != ns // 2 or not (
+            c.is_contiguous() and s.is_contiguous()):
+        raise MkError(f"W4Weight: expected {nc} bytes of codes and {ns // 2} bf16 scales, contiguous")
 
 
 def quantize_w4(weight: torch.Tensor, group: int = 128) -> W4Weight:
     """weight (N, K) bf16 -> 4-bit codes in [-7, 7] under a bf16 scale amax / 7 per row and `group` (32, 64 or 128)
     values of K.  Any N and K; rows may be strided.  A group with a NaN or an infinity gets a NaN scale."""
     lib = load()
-    _need_rows(weight, "weight", (BF16,))
-    n, k = weight.shape
-    nc, ns = _w4_sizes(n, k, int(group))
-    with _on(weight):
-        codes = torch.empty(nc, dtype=torch.uint8, device=weight.device)
-        scales = torch.empty(ns // 2, dtype=BF16, device=weight.device)
-        check(lib.mk_w4_quantize(_adr(weight), weight.stride(0), n, k, group, _adr(codes), _adr(scales), _raw_stream()),
-              "mk_w4_quantize")
-    return W4Weight(codes, scales, n, k, int(group))
+    n, k, ld = _need_rows(weight, "weight", (BF16,))
+    group = int(group)
+    nc, ns = _w4_sizes(n, k, group)
+    codes, scales = weight.new_empty(nc, dtype=torch.uint8), weight.new_empty(ns // 2)
+    _call(weight, lib.mk_w4_quantize, "mk_w4_quantize", _adr(weight), ld, n, k, group, _adr(codes), _adr(scales))
+    return W4Weight(codes, scales, n, k, group)
 
 
 def dequantize_w4(w: W4Weight, dtype: torch.dtype = BF16) -> torch.Tensor:
     """The values a W4Weight stands for: (N, K) f32 (exact) or bf16 (rounded once)."""
     lib = load()
-    _need_w4(w)
-    if dtype not in (BF16, torch.float32):
+    if dtype not in (BF16, F32):
         raise MkError(f"dequantize_w4: dtype {dtype}, expected bf16 or f32")
-    with _on(w.codes):
-        out = torch.empty((w.n, w.k), dtype=dtype, device=w.codes.device)
-        check(lib.mk_w4_dequantize(_adr(w.codes), _adr(w.scales), w.n, w.k, w.group, _adr(out), int(dtype != BF16), w.k,
-                                   _raw_stream()), "mk_w4_dequantize")
+    _need_w4(w)
+    out = w.scales.new_empty((w.n, w.k), dtype=dtype)
+    _call(out, lib.mk_w4_dequantize, "mk_w4_dequantize", _adr(w.codes), _adr(w.scales), w.n, w.k, w.group, _adr(out),
+          int(dtype != BF16), w.k)
     return out
 
 
 def gemm_w4(x: torch.Tensor, w: W4Weight, dtype: torch.dtype = BF16, out: torch.Tensor | None = None) -> torch.Tensor:
     """x (M, K) bf16 @ w (N, K)^T with 4-bit weights, f32 accumulation -> (M, N) bf16 or f32 (include/mk.h, mk_gemm_w4).
 
-    For few rows: the weights are read once per 64 rows of x.  x and `out` may have strided rows."""
+    For few rows: the weights are read once per 64 rows of x.  x and `out` may have strided rows; `out` must not overlap x
+    or the weight.  A row's result is the same in every batch."""
     lib = load()
     _need_w4(w)
-    _need_rows(x, "x", (BF16,), w.k)
-    M = x.shape[0]
+    M, _, ldx = _need_rows(x, "x", (BF16,), w.k)
     if out is None:
-        if dtype not in (BF16, torch.float32):
+        if dtype not in (BF16, F32):
             raise MkError(f"gemm_w4: dtype {dtype}, expected bf16 or f32")
+        _same_device(x, w=w.codes)
+        out = x.new_empty((M, w.n), dtype=dtype)
+        ldo = w.n
     else:
-        _need_rows(out, "out", (BF16, torch.float32), w.n)
-        if out.shape[0] != M:
-            raise MkError(f"out: {out.shape[0]} rows, expected {M}")
-    _same_device(x, w=w.codes, out=out)
-    with _on(x):
-        if out is None:
-            out = torch.empty((M, w.n), dtype=dtype, device=x.device)
-        check(lib.mk_gemm_w4(_adr(x), x.stride(0), _adr(w.codes), _adr(w.scales), M, w.n, w.k, w.group, _adr(out),
-                             int(out.dtype != BF16), out.stride(0), _raw_stream()), "mk_gemm_w4")
+        rows, _, ldo = _need_rows(out, "out", (BF16, F32), w.n)
+        if rows != M:
+            raise MkError(f"out: {rows} rows, expected {M}")
+        _same_device(x, w=w.codes, out=out)
+    _call(x, lib.mk_gemm_w4, "mk_gemm_w4", _adr(x), ldx, _adr(w.codes), _adr(w.scales), M, w.n, w.k, w.group, _adr(out),
+          int(out.dtype != BF16), ldo)
     return out
 
 

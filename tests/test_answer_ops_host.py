@@ -153,8 +153,10 @@ def test_w4_cpu_tensors():
     w = ops.W4Weight(z, z.bfloat16(), 4, 64, 64)
     with pytest.raises(_lib.MkError, match="dtype"):
         ops.dequantize_w4(w, dtype=torch.float16)
-    with pytest.raises(_lib.MkError, match="GPU tensor"):
+    with pytest.raises(_lib.MkError, match="GPU tensors"):
         ops.gemm_w4(torch.zeros(1, 64, dtype=torch.bfloat16), w)
+    with pytest.raises(_lib.MkError, match="group"):
+        ops.gemm_w4(torch.zeros(1, 64, dtype=torch.bfloat16), w._replace(group=48))
 
 
 def test_candidate_ids():

@@ -187,6 +187,10 @@ def test_refusals():
                      (lambda: ops.quantize_w4(x.T, 32), "contiguous"),
                      (lambda: ops.quantize_w4(x[:0], 32), "empty"),
                      (lambda: ops.gemm_w4(x[:, :255], q), "columns"),
+                     (lambda: ops.gemm_w4(x, q._replace(n=1000)), "bytes of codes"),
+                     (lambda: ops.gemm_w4(x, q._replace(scales=q.scales[:-1])), "bf16 scales"),
+                     (lambda: ops.gemm_w4(x, q._replace(scales=q.scales.cpu())), "one device"),
+                     (lambda: ops.dequantize_w4(q._replace(k=4000)), "bytes of codes"),
                      (lambda: ops.gemm_w4(x.half(), q), "expected 2 dimensions"),
                      (lambda: ops.gemm_w4(x.expand(2, 4, 256), q), "expected 2 dimensions"),
                      (lambda: ops.gemm_w4(x[:1].expand(4, 256), q), "overlap"),
