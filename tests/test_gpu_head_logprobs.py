@@ -126,6 +126,27 @@ def test_many_rows():
     _check(h, w, ids)
 
 
+@pytest.mark.parametrize("T", [3, 70])
+def test_large_weight(T):
+    """A head of more than 4 GiB: the vocabulary in slices, given tokens on both sides of the cut."""
+    V, H = 270000, 8192
+    h, _, _ = _inputs(T, H, 1, 1, seed=3)
+    w = torch.empty((V, H), device=DEV, dtype=BF16)
+    for part in w.split(30000):
+        part.copy_(0.01 * torch.randn(part.shape, device=DEV))
+    cut = ((1 << 32) - 1) // (2 * H) // 256 * 256
+    ids = torch.tensor([[0, cut - 1, cut, V - 1]] * T, device=DEV)
+    x = torch.cat([torch.mm(h.float(), part.float().T.contiguous()) for part in w.split(30000)], 1).double()
+    from minicpm5_mk import ops
+
+    r = ops.lm_head_logprobs(h, w, ids)
+    lp = torch.log_softmax(x, -1)
+    # both sides' logits are f32 sums of 8192 products: relative errors of a few 2^-24 sqrt(8192) in norm
+    assert float((r.token_logprobs.double() - lp.gather(1, ids)).norm()) <= 4e-6 * float(lp.gather(1, ids).norm())
+    assert float((r.logsumexp.double() - torch.logsumexp(x, -1)).abs().max()) <= 1e-4
+    assert float((r.entropy.double() + (lp.exp() * lp).sum(-1)).abs().max()) <= 1e-4
+
+
 def test_refusals():
     from minicpm5_mk import ops
 

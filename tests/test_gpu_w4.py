@@ -117,7 +117,7 @@ def _check_gemm(x, q, dtype, got=None):
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("m,n,k", [
     (1, 1, 1), (1, 16, 128), (2, 17, 33), (3, 100, 1000), (16, 256, 1536), (17, 130, 1100), (32, 64, 4608), (33, 40, 200),
-    (64, 1000, 777), (5, 8192, 1536), (1, 1536, 4608), (1, 33000, 256), (40, 70000, 128), (65, 48, 300), (130, 100, 520),
+    (64, 1000, 777), (5, 8192, 1536), (1, 1536, 4608), (1, 33000, 256), (40, 70000, 128), (65, 48, 300), (130, 100, 520), (5000, 20, 40),
 ])
 def test_gemm(m, n, k, group):
     from minicpm5_mk import ops
