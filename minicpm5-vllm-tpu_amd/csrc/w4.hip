@@ -7,8 +7,9 @@
 //
 // Layout.  Blocks of 16 rows x 128 values of K, 1 KB, [row block][K block]: lane l of a wave has the 16 bytes at 16 l,
 // word t of them row l % 16, values 32 t + 8 (l / 16) .. + 7 -- operand A of the 16x16x32 MFMA t of the block, so the
-// product reads weights as whole-wave 1 KB loads and moves nothing between lanes.  Value 2 p of a word is its nibble p,
-// value 2 p + 1 its nibble 4 + p: one shift and one and-or make a bf16 pair.  Rows and values past N and K hold code 0
+// product reads weights as whole-wave 1 KB loads and moves nothing between lanes.  Value 2 p of a word is nibble p, value
+// 2 p + 1 nibble 4 + p of the word rotated right by 3: rotated right by 4 p the word has both where the mantissas of two
+// bf16 take them, so a rotation (none for p = 0) and one and-or make a pair.  Rows and values past N and K hold code 0
 // (scale 0).  Scales: [row block][K block][row / 4][group of the block][row % 4], so a lane's four accumulator rows have
 // theirs next to each other.
 #include <algorithm>
@@ -87,7 +88,7 @@ __global__ __launch_bounds__(256) void w4_quantize_kernel(const uint16_t* __rest
         const int u = (int)fminf(fmaxf(rintf(c), -7.f), 7.f) + 8;
         word |= (uint32_t)u << (4 * (i / 2) + 16 * (i % 2));
       }
-      out[t] = word;
+      out[t] = __builtin_rotateleft32(word, 3);
     }
   }
   reinterpret_cast<u32x4*>(codes)[(size_t)b * 64 + lane] = out;
@@ -114,11 +115,12 @@ __global__ __launch_bounds__(256) void w4_dequantize_kernel(const uint8_t* __res
   const uint16_t* sp = scales + (size_t)b * W4_ROWS * GPB + (r >> 2) * 4 * GPB + (r & 3);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
+    const uint32_t word = __builtin_rotateright32(c[t], 3);
     const float s = bf2f(sp[4 * (t * GPB / 4)]);
     const int k = kb * W4_K + 32 * t + 8 * kq;
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)((int)(c[t] >> (4 * (i / 2) + 16 * (i % 2)) & 15) - 8) * s;
+    for (int i = 0; i < 8; ++i) v[i] = (float)((int)(word >> (4 * (i / 2) + 16 * (i % 2)) & 15) - 8) * s;
     if constexpr (F32) {
       float* o = static_cast<float*>(out) + n * ldo + k;
       typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -153,7 +155,7 @@ __global__ __launch_bounds__(256) void w4_dequantize_kernel(const uint8_t* __res
 // more MFMAs, which no longer hide behind the stream: 48 rows 38.7 us, 64 rows 51.2 (K = 2048: 40 rows 48, 64 rows 56).
 // Small weights are bound by latency, one pass of loads after another (1536 x 4608, one row 5.3 us).
 //
-// A code becomes the bf16 number 16 + u = c + 24: 0x4180 with u in the mantissa, exact.  The 24 too much are taken off
+// A code becomes the bf16 number 16 + u = c + 24: 0x4180 with u in mantissa bits 3 - 6, exact.  The 24 too much are taken off
 // before they are added: the accumulators of a group start at -24 sum x over the group (f32), so a group's sum is
 // sum c x, with roundings relative to 24 |sum x| at most; it is scaled by s (f32) into the row's total.
 //
@@ -166,9 +168,9 @@ constexpr int w4_waves(int mg) { return mg == 1 ? 8 : 16; }
 constexpr int w4_xb(int mg) { return w4_waves(mg) * 8192; }   // LDS bytes of x, and of its sums (groups of 32)
 constexpr int w4_sb(int mg) { return w4_xb(mg) / 16; }
 
-__device__ inline uint32_t pair_bf16(uint32_t w, int p) {
-  const uint32_t v = p == 0 ? w << 3 : w >> (4 * p - 3);
-  return (v & 0x00780078u) | 0x41804180u;
+// mask: 0x00780078, the mantissa bits of the codes; one: 0x41804180, bf16 16.0 twice
+__device__ inline uint32_t pair_bf16(uint32_t w, int p, uint32_t mask, uint32_t one) {
+  return (__builtin_rotateright32(w, 4 * p) & mask) | one;
 }
 
 template <int MG, int R, int GROUP>
@@ -193,6 +195,10 @@ __global__ __launch_bounds__(64 * w4_waves(MG), 4) void w4_gemm_kernel(W4GemmArg
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int m = 0; m < MG; ++m) tot[r][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // kept in registers the compiler cannot see through: as literals they would make an and and an or of the and-or
+  uint32_t mask = 0x00780078u, one = 0x41804180u;
+  asm volatile("" : "+s"(mask), "+v"(one));
 
   typedef uint16_t SC __attribute__((ext_vector_type(4 * GPB)));
   u32x4 cw[R];
@@ -272,7 +278,7 @@ __global__ __launch_bounds__(64 * w4_waves(MG), 4) void w4_gemm_kernel(W4GemmArg
 #pragma unroll
           for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int p = 0; p < 4; ++p) av[r][p] = pair_bf16(cb[r][t], p);
+            for (int p = 0; p < 4; ++p) av[r][p] = pair_bf16(cb[r][t], p, mask, one);
 #pragma unroll
           for (int m = 0; m < MG; ++m) {
             const u32x4 bv = *reinterpret_cast<const u32x4*>(smem + lb * RA * 256 + xoff[t] + m * 4096);
