@@ -3,7 +3,7 @@
 // Format.  W (N, K): along K every row is cut into groups of `group` (32, 64 or 128) values, the last one filled up with
 // zeros; group g of row n has the scale s = bf16(amax / 7) and codes c = round_half_even(w / s) in [-7, 7], W ~ c s.
 // A group whose amax / 7 is below the smallest normal number has s = 0 and codes 0; a group with an infinity or a NaN
-// has s = NaN.  Stored are u = c + 8 (4 bits) and s (bf16).
+// has s = NaN.  Stored are s (bf16) and 4 bits u a value, 8 + c at even k and 8 - c at odd k (the product's reason).
 //
 // Layout.  Blocks of 16 rows x 128 values of K, 1 KB, [row block][K block]: lane l of a wave has the 16 bytes at 16 l,
 // word t of them row l % 16, values 32 t + 8 (l / 16) .. + 7 -- operand A of the 16x16x32 MFMA t of the block, so the
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256) void w4_quantize_kernel(const uint16_t* __rest
         const float v = bf2f(raw[t][i]) * f;
         float c = v * inv;
         c = fmaf(fmaf(-c, sf, v), inv, c);
-        const int u = (int)fminf(fmaxf(rintf(c), -7.f), 7.f) + 8;
+        const int q = (int)fminf(fmaxf(rintf(c), -7.f), 7.f), u = i % 2 ? 8 - q : 8 + q;
         word |= (uint32_t)u << (4 * (i / 2) + 16 * (i % 2));
       }
       out[t] = __builtin_rotateleft32(word, 3);
@@ -120,7 +120,10 @@ __global__ __launch_bounds__(256) void w4_dequantize_kernel(const uint8_t* __res
     const int k = kb * W4_K + 32 * t + 8 * kq;
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)((int)(word >> (4 * (i / 2) + 16 * (i % 2)) & 15) - 8) * s;
+    for (int i = 0; i < 8; ++i) {
+      const int u = word >> (4 * (i / 2) + 16 * (i % 2)) & 15;
+      v[i] = (float)(i % 2 ? 8 - u : u - 8) * s;
+    }
     if constexpr (F32) {
       float* o = static_cast<float*>(out) + n * ldo + k;
       typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -151,13 +154,15 @@ __global__ __launch_bounds__(256) void w4_dequantize_kernel(const uint8_t* __res
 // ------------------------------------------------------------------------------------------------ product
 // y (M, N) = x (M, K) (c s)^T, f32 accumulation.  For few rows the weight stream is the bound: the 130560 x 1536 head takes
 // 22.3 us for one row (4.65 TB/s, what a large copy reaches), 27 for 16.  Beyond, a block of 16 x 128 weights costs a wave
-// 32 VALU operations of unpacking, and per group and 16 rows of x four to start, four to scale the accumulators and two or
+// 28 VALU operations of unpacking, and per group and 16 rows of x four to start, four to scale the accumulators and two or
 // more MFMAs, which no longer hide behind the stream: 48 rows 38.7 us, 64 rows 51.2 (K = 2048: 40 rows 48, 64 rows 56).
 // Small weights are bound by latency, one pass of loads after another (1536 x 4608, one row 5.3 us).
 //
-// A code becomes the bf16 number 16 + u = c + 24: 0x4180 with u in mantissa bits 3 - 6, exact.  The 24 too much are taken off
-// before they are added: the accumulators of a group start at -24 sum x over the group (f32), so a group's sum is
-// sum c x, with roundings relative to 24 |sum x| at most; it is scaled by s (f32) into the row's total.
+// u becomes a bf16 number by standing in mantissa bits 3 - 6 of 16.0 at even k and of -16.0 at odd k: 16 + u = 24 + c and
+// -(16 + u) = c - 24, exact.  What is too much is 24 d, d the even x less the odd ones of a group, and taken off before
+// it is added: the group's accumulators start at -24 d (f32) and end at sum c x, which is scaled by s (f32) into the row's
+// total.  The roundings between are relative to 24 |d|, which x of one sign do not raise (with + 24 at every k, x uniform
+// in 0 .. 1 and groups of 128 gave 2.2e-6 of the result's norm).
 //
 // x is staged in LDS, as many blocks of 128 values of K at a time as fit (zeros past K), each block its rows of 256 bytes,
 // 16-byte piece p of row m at p ^ (m % 16) so that the 16 rows of an operand read are on distinct banks; its group sums are
@@ -168,7 +173,7 @@ constexpr int w4_waves(int mg) { return mg == 1 ? 8 : 16; }
 constexpr int w4_xb(int mg) { return w4_waves(mg) * 8192; }   // LDS bytes of x, and of its sums (groups of 32)
 constexpr int w4_sb(int mg) { return w4_xb(mg) / 16; }
 
-// mask: 0x00780078, the mantissa bits of the codes; one: 0x41804180, bf16 16.0 twice
+// mask: 0x00780078, the mantissa bits of the codes; one: 0xc1804180, bf16 16.0 and -16.0
 __device__ inline uint32_t pair_bf16(uint32_t w, int p, uint32_t mask, uint32_t one) {
   return (__builtin_rotateright32(w, 4 * p) & mask) | one;
 }
@@ -197,7 +202,7 @@ __global__ __launch_bounds__(64 * w4_waves(MG), 4) void w4_gemm_kernel(W4GemmArg
     for (int m = 0; m < MG; ++m) tot[r][m] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // kept in registers the compiler cannot see through: as literals they would make an and and an or of the and-or
-  uint32_t mask = 0x00780078u, one = 0x41804180u;
+  uint32_t mask = 0x00780078u, one = 0xc1804180u;
   asm volatile("" : "+s"(mask), "+v"(one));
 
   typedef uint16_t SC __attribute__((ext_vector_type(4 * GPB)));
@@ -245,7 +250,7 @@ __global__ __launch_bounds__(64 * w4_waves(MG), 4) void w4_gemm_kernel(W4GemmArg
         *reinterpret_cast<u32x4*>(smem + ((p >> 4) * RA + m) * 256 + ((p ^ m) & 15) * 16) = __builtin_bit_cast(u32x4, v[q]);
         float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += bf2f(v[q][e]);
+        for (int e = 0; e < 8; e += 2) s += bf2f(v[q][e]) - bf2f(v[q][e + 1]);
 #pragma unroll
         for (int o = 1; o < GROUP / 8; o <<= 1) s += __shfl_xor(s, o);   // ppr is a multiple of 16: whole groups
         if (p % (GROUP / 8) == 0) sums[(p / (GROUP / 8)) * RA + m] = -24.f * s;

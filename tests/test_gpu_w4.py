@@ -128,6 +128,24 @@ def test_gemm(m, n, k, group):
     _check_gemm(x, q, BF16)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_gemm_one_sided_x(group):
+    """x of one sign, whose sums are far larger than the result: no more rounding than 16 half steps of the result's norm
+    (an f32 product over the weights' values measures 2)."""
+    from minicpm5_mk import ops
+
+    q = ops.quantize_w4(_weight(5000, 1536), group)
+    w = ops.dequantize_w4(q, dtype=F32).double()
+    g = torch.Generator(device=DEV)
+    g.manual_seed(8)
+    for x in (torch.rand((6, 1536), generator=g, device=DEV), 3 + torch.randn((6, 1536), generator=g, device=DEV),
+              torch.exp(1.5 * torch.randn((6, 1536), generator=g, device=DEV))):
+        x = x.to(BF16)
+        want = torch.mm(x.double(), w.T.contiguous())
+        err = ops.gemm_w4(x, q, dtype=F32).double() - want
+        assert float(err.norm()) <= 16 * 2.0 ** -24 * float(want.norm())
+
+
 def test_gemm_rows_alone():
     """A row's result does not depend on the other rows or how many they are: one block or several a wave, K dealt out or
     not."""
