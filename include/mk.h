@@ -259,6 +259,7 @@ int mk_lm_head(const void* hidden, const void* lm_head, int B, int H, int V, flo
  *   token_lp (T, n_ids) = (x[id] - m) - ln S of the given tokens ids (T, n_ids), int32 or int64 (ids64 != 0)
  *   ranks (T, n_ids) = 1 + the number of tokens before id in the order (logit descending, index ascending)
  *   top_lp, top_ids (T, top): the first `top` tokens of that order
+ * ln S is made from the sum without its largest term: the log probability of an all but certain token is not rounded away.
  * An id outside [0, V) has log probability -inf and rank -1.  A row of nothing but -inf has lse and log
  * probabilities -inf and entropy 0.  A row with a NaN or +inf has no distribution: its numbers are NaN, its ranks
  * and top_ids -1.  n_ids and top may be 0 (at most MK_LOGPROBS_MAX each, top <= V), their pointers are then unused.

@@ -5,7 +5,10 @@
 //   lse = m + ln S,  entropy = ln S - U / S,  log p(i) = (x_i - m) - ln S
 //   rank(i) = 1 + #{x_j > x_i} + #{j < i : x_j = x_i}: i's place in the order (value descending, index ascending),
 //   the order of the k best as well.
-// (x_i - m) - ln S, not x_i - lse: a row whose values are all large (masked to the type's lowest value) keeps ln S.
+// (x_i - m) - ln S, not x_i - lse: a row whose values are all large (masked to the type's lowest value) keeps ln S.  ln S
+// is log1p(S - 1) with S - 1 summed without the row's largest term: where one token is all but certain, an f32 S near 1
+// would lose what that token's log probability and the entropy consist of (a token 12 above 32768 others: relative error
+// 1e-3 that way, 3e-7 this way).
 //
 // One pass over the row: every lane keeps a running m, S, U, rescaled once per 16 values, and every wave the k
 // best of what it has seen.  Bytes bound it: 16 values of a lane cost about 12 VALU operations each, one of them a
@@ -61,11 +64,13 @@ struct Stat {
     s *= f;
     m = mn;
   }
-  // the wave's lanes as one
-  __device__ void reduce() {
-    raise(wave_max(m));
-    s = wave_sum(s);
-    u = wave_sum(u);
+  // raises every lane to the wave's maximum; the first lane with values that holds it (0 where none has any)
+  __device__ int join() {
+    const float lm = m;
+    const bool some = s > 0.f;
+    raise(wave_max(lm));
+    const unsigned long long mask = __ballot(some && lm == m);
+    return mask ? __builtin_ctzll(mask) : 0;
   }
 };
 
@@ -181,7 +186,7 @@ struct Load<_Float16> {
   }
 };
 
-// Workspace of one (row, split): m, s, u, unused; of each given token the count of values above it and, from the split
+// Workspace of one (row, split): m, s, u, s without its largest term; of each given token the count of values above it and, from the split
 // that holds it, its value; the list of k entries, 8-byte aligned.
 __host__ __device__ inline size_t part_floats(int n_ids, int k) { return 4 + 2 * (size_t)n_ids + 2 * (size_t)k; }
 
@@ -190,24 +195,32 @@ struct RowShared {
   u64 list[WAVES][LP_CAP];   // by wave
   u64 all[WAVES * 64];       // what is left of them at the end, in any order
   float m[WAVES], s[WAVES], u[WAVES];
+  float sx[WAVES];           // s without the first lane that holds m
+  float rest;                // terms of that lane beside its largest
   int n;                     // entries of all
   float gmax[64];            // largest value seen by each of 64 groups of lanes
   int rank[WAVES][LP_MAX_IDS];
 };
 
-// The waves' statistics as one, in every thread.
+// The waves' statistics as one, in every thread; `first`: the first wave that holds the maximum, sx: s without that
+// wave's first lane that does.
 template <int WAVES>
-__device__ inline Stat merge_stats(const RowShared<WAVES>& sh) {
+__device__ inline Stat merge_stats(const RowShared<WAVES>& sh, int& first, float& sx) {
   Stat st;
 #pragma unroll
   for (int o = 0; o < WAVES; ++o) st.m = fmaxf(st.m, sh.m[o]);
+  first = -1;
+  sx = 0.f;
 #pragma unroll
   for (int o = 0; o < WAVES; ++o) {
     Stat x;
     x.m = sh.m[o]; x.s = sh.s[o]; x.u = sh.u[o];
+    const bool is = first < 0 && x.s > 0.f && x.m == st.m;
+    first = is ? o : first;
     x.raise(st.m);
     st.s += x.s;
     st.u += x.u;
+    sx += is ? sh.sx[o] : x.s;
   }
   return st;
 }
@@ -238,23 +251,22 @@ __device__ inline void best_of_all(const RowShared<WAVES>& sh, int k, F put) {
   }
 }
 
-// The row's outputs: st its statistics, lane j of wave 0 given token j (id < 0: outside the vocabulary) with its
-// value and the count of values above it.
+// The row's outputs: its statistics, r the sum without its largest term.  ln S = log1p(r): where one token is all but
+// certain, 1 + r in f32 would lose r, which its log probability and the entropy are made of.
 struct RowOut {
   bool nan, empty;
-  Stat st;
-  float ls;
-  __device__ RowOut(const Stat& s) : st(s) {
-    nan = !(s.s == s.s);     // an infinite logit makes s NaN as well
-    empty = s.s == 0.f;
-    ls = logf(s.s);
+  float m, u, s, ls;
+  __device__ RowOut(const Stat& st, float r) : m(st.m), u(st.u), s(st.s) {
+    nan = !(s == s);         // an infinite logit makes s NaN as well
+    empty = s == 0.f;
+    ls = log1pf(r);
   }
   __device__ float lp(float v) const {
-    return nan ? __builtin_nanf("") : empty ? neg_inf() : (v - st.m) - ls;
+    return nan ? __builtin_nanf("") : empty ? neg_inf() : (v - m) - ls;
   }
   __device__ void stats(const LogprobArgs& a, int row) const {
-    a.lse[row] = nan ? __builtin_nanf("") : empty ? neg_inf() : st.m + ls;
-    a.entropy[row] = nan ? __builtin_nanf("") : empty ? 0.f : ls - st.u / st.s;
+    a.lse[row] = nan ? __builtin_nanf("") : empty ? neg_inf() : m + ls;
+    a.entropy[row] = nan ? __builtin_nanf("") : empty ? 0.f : ls - u / s;
   }
   __device__ void token(const LogprobArgs& a, int row, int j, bool in, float v, int above) const {
     const size_t o = (size_t)row * a.n_ids + j;
@@ -404,11 +416,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 6) void logprob_rows_
     }
   }
 
-  st.reduce();
+  const int holder = st.join();
+  const float sx = wave_sum(lane == holder ? 0.f : st.s);
+  st.s = wave_sum(st.s);
+  st.u = wave_sum(st.u);
   if (lane == 0) {
     sh.m[w] = st.m;
     sh.s[w] = st.s;
     sh.u[w] = st.u;
+    sh.sx[w] = sx;
   }
   if (a.top) give_list(sh, top);
   if (lane < a.n_ids) sh.rank[w][lane] = above;
@@ -418,9 +434,29 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 6) void logprob_rows_
 #pragma unroll
     for (int o = 0; o < WAVES; ++o) above += sh.rank[o][lane];
   }
-  const Stat all = merge_stats(sh);
+  int fw;
+  float r;
+  const Stat all = merge_stats(sh, fw, r);
+  if (all.s < 2.f && all.s > 0.f) {
+    // One term outweighs the others: its lane's sum has lost what they are.  The wave adds them again without it.
+    if (w == fw) {
+      float p = 0.f;
+      const int mine = c0 + w * LP_TILE;
+      for (int q = lane; q < (c1 - mine + WAVES * LP_TILE - 1) / (WAVES * LP_TILE) * LP_E; q += 64) {
+        const int e = q % LP_E, i = mine + q / LP_E * (WAVES * LP_TILE) + (e / VEC) * 64 * VEC + holder * VEC + e % VEC;
+        const float v = i < c1 ? L::f(x[i]) : neg_inf();
+        p += v < all.m ? fast_exp2((v - all.m) * LOG2E) : 0.f;
+      }
+      p = wave_sum(p);
+      if (lane == 0) sh.rest = p;
+    }
+    __syncthreads();
+    r += sh.rest;
+  } else {
+    r = all.s - 1.f;
+  }
   if constexpr (!SPLIT) {
-    const RowOut out(all);
+    const RowOut out(all, r);
     if (threadIdx.x == 0) out.stats(a, row);
     if (w == 0 && lane < a.n_ids) out.token(a, row, lane, id >= 0, iv, above);
     if (out.nan) {
@@ -434,6 +470,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 6) void logprob_rows_
       p[0] = all.m;
       p[1] = all.s;
       p[2] = all.u;
+      p[3] = r;
     }
     if (w == 0 && lane < a.n_ids) {
       reinterpret_cast<int*>(p)[4 + 2 * lane] = above;
@@ -453,15 +490,14 @@ __global__ __launch_bounds__(256) void logprob_merge_kernel(LogprobArgs a, int s
   const size_t pf = part_floats(a.n_ids, a.top);
   const float* p = part + (size_t)row * splits * pf;
 
+  // a thread a split (at most one workgroup a CU splits a row); the first split that holds the maximum gives its sum
+  // without it
   Stat st;
-  for (int i = threadIdx.x; i < splits; i += 256) {
-    Stat x;
-    x.m = p[i * pf]; x.s = p[i * pf + 1]; x.u = p[i * pf + 2];
-    const float mn = fmaxf(st.m, x.m);
-    st.raise(mn);
-    x.raise(mn);
-    st.s += x.s;
-    st.u += x.u;
+  float sx = 0.f;
+  if (threadIdx.x < splits) {
+    const float* e = p + threadIdx.x * pf;
+    st.m = e[0]; st.s = e[1]; st.u = e[2];
+    sx = e[3];
   }
   int above = 0;
   bool in = false;
@@ -491,14 +527,21 @@ __global__ __launch_bounds__(256) void logprob_merge_kernel(LogprobArgs a, int s
     }
     give_list(sh, top);
   }
-  st.reduce();
+  const int holder = st.join();
+  sx = wave_sum(lane == holder ? sx : st.s);
+  st.s = wave_sum(st.s);
+  st.u = wave_sum(st.u);
   if (lane == 0) {
     sh.m[w] = st.m;
     sh.s[w] = st.s;
     sh.u[w] = st.u;
+    sh.sx[w] = sx;
   }
   __syncthreads();
-  const RowOut out(merge_stats(sh));
+  int fw;
+  float r;
+  const Stat all = merge_stats(sh, fw, r);
+  const RowOut out(all, r);
   if (threadIdx.x == 0) out.stats(a, row);
   if (w == 0 && lane < a.n_ids) out.token(a, row, lane, in, iv, above);
   if (out.nan) {

@@ -138,6 +138,40 @@ def test_masks(T, dtype):
     assert float(r.entropy[0]) == 0.0 and float(r.entropy[2]) == 0.0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,V", [(3, 1), (6, 700), (3, 32768), (2, 130560), (40, 70001), (300, 33000), (1000, 20000)])
+def test_certain_tokens(T, V, dtype):
+    """Rows where one token outweighs all others: its log probability and the entropy are sums of the others' small
+    terms, each off by its exponent's roundings (|d| log2 e at 2^-24 twice, |d| <= 60) and the exponential's 2^-23, then
+    a few hundred additions of one sign."""
+    from minicpm5_mk import ops
+
+    x = _logits(T, V, dtype, scale=1.0)
+    at = _ids(T, V, 1, seed=V)
+    for up in (12.0, 20.0, 40.0):
+        x.scatter_(1, at, up)
+        r = ops.logprobs(x, at, top=1)
+        d = x.cpu().double() - up
+        rest = d.exp().scatter(1, at.cpu(), 0.0).sum(-1)
+        lp, ent = -torch.log1p(rest), torch.log1p(rest) - (d.exp() * d).sum(-1) / (1 + rest)
+        tol = (2 * 60 * 1.5 + 2 + 400) * 2.0 ** -24
+        assert ((r.token_logprobs[:, 0].cpu().double() - lp).abs() <= tol * lp.abs()).all()
+        assert ((r.entropy.cpu().double() - ent).abs() <= tol * ent.abs()).all()
+        assert torch.equal(r.top_ids.long(), at) and (r.ranks == 1).all()
+        assert torch.equal(r.top_logprobs, r.token_logprobs)
+
+
+@pytest.mark.parametrize("T", [2, 100, 300, 1000])
+def test_one_lowest_value(T):
+    """One finite token, the type's lowest, among -inf: certain."""
+    from minicpm5_mk import ops
+
+    x = torch.full((T, 40000), -INF, device=DEV)
+    x[:, 39001] = torch.finfo(torch.float32).min
+    r = ops.logprobs(x, torch.full((T, 1), 39001, device=DEV), top=2)
+    assert (r.token_logprobs == 0).all() and (r.entropy == 0).all() and (r.top_ids == torch.tensor([39001, 0], device=DEV)).all()
+
+
 def test_ids_outside():
     x = _logits(4, 5000, torch.float32)
     ids = torch.tensor([[-1, 0, 4999], [5000, -100, 1], [2 ** 40, -2 ** 40, 2], [3, 3, 3]], device=DEV)
