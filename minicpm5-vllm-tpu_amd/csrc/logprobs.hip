@@ -195,15 +195,13 @@ struct RowShared {
   u64 list[WAVES][LP_CAP];   // by wave
   u64 all[WAVES * 64];       // what is left of them at the end, in any order
   float m[WAVES], s[WAVES], u[WAVES];
-  float sx[WAVES];           // s without the first lane that holds m
-  float rest;                // terms of that lane beside its largest
+  float rest;                // the s of the wave that holds the maximum without it
   int n;                     // entries of all
   float gmax[64];            // largest value seen by each of 64 groups of lanes
   int rank[WAVES][LP_MAX_IDS];
 };
 
-// The waves' statistics as one, in every thread; `first`: the first wave that holds the maximum, sx: s without that
-// wave's first lane that does.
+// The waves' statistics as one, in every thread; `first`: the first wave that holds the maximum, sx: s without that wave's.
 template <int WAVES>
 __device__ inline Stat merge_stats(const RowShared<WAVES>& sh, int& first, float& sx) {
   Stat st;
@@ -220,7 +218,7 @@ __device__ inline Stat merge_stats(const RowShared<WAVES>& sh, int& first, float
     x.raise(st.m);
     st.s += x.s;
     st.u += x.u;
-    sx += is ? sh.sx[o] : x.s;
+    sx += is ? 0.f : x.s;
   }
   return st;
 }
@@ -417,14 +415,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 6) void logprob_rows_
   }
 
   const int holder = st.join();
-  const float sx = wave_sum(lane == holder ? 0.f : st.s);
+  const float own = st.s;                  // the lane's
   st.s = wave_sum(st.s);
   st.u = wave_sum(st.u);
   if (lane == 0) {
     sh.m[w] = st.m;
     sh.s[w] = st.s;
     sh.u[w] = st.u;
-    sh.sx[w] = sx;
   }
   if (a.top) give_list(sh, top);
   if (lane < a.n_ids) sh.rank[w][lane] = above;
@@ -437,10 +434,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 6) void logprob_rows_
   int fw;
   float r;
   const Stat all = merge_stats(sh, fw, r);
-  if (all.s < 2.f && all.s > 0.f) {
-    // One term outweighs the others: its lane's sum has lost what they are.  The wave adds them again without it.
+  if (all.s < 1.25f && all.s > 0.f) {
+    // One term outweighs the others, and its lane's sum has lost what they are (above 1.25 s - 1 is exact to 4e-7).  Its
+    // wave adds them again without it.
     if (w == fw) {
-      float p = 0.f;
+      float p = lane == holder ? 0.f : own;
       const int mine = c0 + w * LP_TILE;
       for (int q = lane; q < (c1 - mine + WAVES * LP_TILE - 1) / (WAVES * LP_TILE) * LP_E; q += 64) {
         const int e = q % LP_E, i = mine + q / LP_E * (WAVES * LP_TILE) + (e / VEC) * 64 * VEC + holder * VEC + e % VEC;
@@ -485,6 +483,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 6) void logprob_rows_
 // One row from its splits' workspace entries, in a fixed order.  Four waves: the splits are few.
 __global__ __launch_bounds__(256) void logprob_merge_kernel(LogprobArgs a, int splits, const float* part) {
   __shared__ RowShared<4> sh;
+  __shared__ float rest[4];                // a wave's s without the largest term
   const int row = blockIdx.x, lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const size_t pf = part_floats(a.n_ids, a.top);
@@ -535,12 +534,13 @@ __global__ __launch_bounds__(256) void logprob_merge_kernel(LogprobArgs a, int s
     sh.m[w] = st.m;
     sh.s[w] = st.s;
     sh.u[w] = st.u;
-    sh.sx[w] = sx;
+    rest[w] = sx;
   }
   __syncthreads();
   int fw;
   float r;
   const Stat all = merge_stats(sh, fw, r);
+  r += fw < 0 ? 0.f : rest[fw];
   const RowOut out(all, r);
   if (threadIdx.x == 0) out.stats(a, row);
   if (w == 0 && lane < a.n_ids) out.token(a, row, lane, in, iv, above);
