@@ -10,9 +10,10 @@
 // would lose what that token's log probability and the entropy consist of (a token 12 above 32768 others: relative error
 // 1e-3 that way, 3e-7 this way).
 //
-// One pass over the row: every lane keeps a running m, S, U, rescaled once per 16 values, and every wave the k
-// best of what it has seen.  Bytes bound it: 16 values of a lane cost about 12 VALU operations each, one of them a
-// quarter-rate exponential, where the vector units could do about 22 per f32 value (11 per 16-bit value) at HBM rate.
+// One pass over the row: every lane keeps a running m, S, U, rescaled once per 16 values, and every wave a list of what
+// may be among the k best.  Bytes bound many rows: (2048, 130560) bf16 121 us, 4.4 TB/s, (1000, 130560) f32 107 us,
+// 4.9 TB/s; a value costs about 12 VALU operations, one of them a quarter-rate exponential, and the vector units are 65 %
+// busy at 16-bit values.  One row is bound by its latencies: loads, bound, listing, merge, 13.5 us at 130560 values.
 #include <algorithm>
 
 #include "kernels.h"
@@ -378,8 +379,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 6) void logprob_rows_
     }
 
     if (a.top) {
-      // Lower bounds of the k-th best, so that few values of a row are ever listed.  64 groups of lanes (a row of 16 of
-      // 16 waves, a quad of 4 waves) publish the largest value each has seen; the k-th largest of those is reached by k
+      // Lower bounds of the k-th best, so that few values of a row are ever listed.  64 groups of lanes (rows of 16 in
+      // 16 waves, halves of them in 8, quads in 4) publish the largest value each has seen; the k-th largest of those is reached by k
       // values: of 16384 random ones about 24 reach the bound for k = 20.  A wave takes a new bound only where a value of
       // its tile passes the last one.  Other waves' entries may be older: lower, still bounds.
       lmax = fmaxf(lmax, tm);
