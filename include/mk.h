@@ -276,7 +276,7 @@ int mk_logprobs(const void* logits, int type, size_t ld, int T, int V, const voi
 
 /* mk_logprobs of the logits hidden (T, H) weight (V, H)^T (bf16, contiguous, f32 accumulation): token_lp, entropy and
  * lse as there, without ranks and alternatives.  Of more than 64 rows no logit is stored, only statistics of 256 tokens
- * of the vocabulary at a time.  H a multiple of 32; hidden, weight and scratch 16-byte aligned; scratch:
+ * of the vocabulary at a time; ln S is then off by a few 1e-7, which is all that is left of an all but certain token.  H a multiple of 32; hidden, weight and scratch 16-byte aligned; scratch:
  * mk_lm_head_logprobs_scratch_bytes bytes (101 MB at most for V = 130560), not shared by calls that overlap.  A row's
  * results may differ in the last bits with the number of rows, as they are made in another order. */
 size_t mk_lm_head_logprobs_scratch_bytes(int T, int V, int n_ids);
